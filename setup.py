@@ -15,7 +15,7 @@ os.environ.setdefault("MAX_JOBS", str(os.cpu_count() or 4))
 
 ROOT = Path(__file__).parent
 CSRC = ROOT / "packbalance_b200" / "csrc"
-SOURCES = ["bindings.cpp", "gemm.cu", "elementwise.cu", "attention.cu", "comm.cu", "fsdp.cu", "noalloc.cu"]
+SOURCES = ["bindings.cpp", "gemm.cu", "elementwise.cu", "layernorm.cu", "attention.cu", "comm.cu", "fsdp.cu", "noalloc.cu"]
 SOURCES = [str((CSRC / s).relative_to(ROOT)) for s in SOURCES]
 # PB_DEBUG_BOUNDS=1 builds the index checks of csrc/common.cuh (PB_BOUNDS_OK) into the
 # kernels: a bad work item, owner rank or token id is reported through the device status
@@ -41,6 +41,10 @@ setup(
         CUDAExtension(
             name="packbalance_b200._C",
             sources=SOURCES,
+            # torch's own (shared) C++ runtime, named explicitly: some g++ installations only find
+            # the static archive, and a second copy of the runtime in the process crashes when an
+            # error message formats a number (its locale facets are never initialised)
+            extra_link_args=["-l:libstdc++.so.6"],
             extra_compile_args={"cxx": ["-O3", "-std=c++17", *DEFINES], "nvcc": NVCC_FLAGS},
         )
     ],
