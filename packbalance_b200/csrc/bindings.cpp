@@ -21,6 +21,11 @@ void swiglu_bwd_packed(at::Tensor dh, at::Tensor gu, at::Tensor dgu);
 std::vector<at::Tensor> rmsnorm_fwd(at::Tensor x, at::Tensor w, double eps, bool out_bf16);
 at::Tensor rmsnorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor rstd, c10::optional<at::Tensor> dres,
                        c10::optional<at::Tensor> dx_bf16, at::Tensor dw_out, bool accumulate_dw);
+std::vector<at::Tensor> add_layernorm_fwd(at::Tensor x, c10::optional<at::Tensor> delta, at::Tensor w,
+                                          c10::optional<at::Tensor> b, double eps, bool out_bf16);
+at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor mean, at::Tensor rstd,
+                         c10::optional<at::Tensor> dres, c10::optional<at::Tensor> dx_bf16, at::Tensor dw_out,
+                         c10::optional<at::Tensor> db_out, bool accumulate);
 at::Tensor swiglu_fwd(at::Tensor g, at::Tensor u);
 std::vector<at::Tensor> swiglu_bwd(at::Tensor g, at::Tensor u, at::Tensor dh);
 void rope_apply(at::Tensor x, at::Tensor pos, at::Tensor cos_t, at::Tensor sin_t, int64_t n_rope_cols,
@@ -65,6 +70,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("add_rmsnorm_fwd", &pb::add_rmsnorm_fwd);
   m.def("swiglu_bwd_packed", &pb::swiglu_bwd_packed);
   m.def("rmsnorm_bwd", &pb::rmsnorm_bwd);
+  m.def("add_layernorm_fwd", &pb::add_layernorm_fwd);
+  m.def("layernorm_bwd", &pb::layernorm_bwd);
   m.def("swiglu_fwd", &pb::swiglu_fwd);
   m.def("swiglu_bwd", &pb::swiglu_bwd);
   m.def("rope_apply", &pb::rope_apply);

@@ -13,6 +13,14 @@ def rmsnorm_reference(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torc
     return (xf * inv * weight.float()).to(x.dtype)
 
 
+def layernorm_reference(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, eps: float) -> torch.Tensor:
+    xf = x.float()
+    centred = xf - xf.mean(dim=-1, keepdim=True)
+    inv = torch.rsqrt(centred.square().mean(dim=-1, keepdim=True) + eps)
+    y = centred * inv * weight.float()
+    return (y if bias is None else y + bias.float()).to(x.dtype)
+
+
 def swiglu_reference(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return F.silu(gate) * up
 
