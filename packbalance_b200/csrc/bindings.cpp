@@ -48,6 +48,14 @@ void attn_bwd(at::Tensor qkv, at::Tensor out, at::Tensor dout, at::Tensor lse, a
               at::Tensor doc_end, at::Tensor items, int64_t H, int64_t Hkv, int64_t D, double scale, at::Tensor dqkv,
               at::Tensor dq_acc, at::Tensor dkv_acc, at::Tensor delta, c10::optional<at::Tensor> pos,
               c10::optional<at::Tensor> cos_t, c10::optional<at::Tensor> sin_t);
+at::Tensor ns_orthogonalize(at::Tensor x, int64_t steps, std::vector<double> coef, double eps);
+void muon_update(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, std::vector<at::Tensor> momenta,
+                 std::vector<at::Tensor> shadows, double lr, double mu, bool nesterov, double weight_decay,
+                 int64_t steps, std::vector<double> coef, double eps, c10::optional<at::Tensor> norm, double max_norm,
+                 c10::optional<at::Tensor> hp);
+void adamw_ranges(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, c10::optional<at::Tensor> shadow,
+                  std::vector<int64_t> ranges, at::Tensor norm, at::Tensor skipped, double lr, double b1, double b2,
+                  double eps, double wd, double bc1, double bc2, double max_norm, c10::optional<at::Tensor> hp);
 void comm_bindings(pybind11::module& m);
 void fsdp_bindings(pybind11::module& m);
 
@@ -83,6 +91,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_row_scale", &pb::ce_row_scale);
   m.def("ce_dlogits", &pb::ce_dlogits, "in-place dlogits over kept bf16 logits");
   m.def("adamw_step", &pb::adamw_step);
+  m.def("ns_orthogonalize", &pb::ns_orthogonalize);
+  m.def("muon_update", &pb::muon_update);
+  m.def("adamw_ranges", &pb::adamw_ranges);
   m.def("l2_norm", &pb::l2_norm);
   m.def("status_read", &pb::status_read, pybind11::arg("dev"), pybind11::arg("clear") = true);
   m.def("attn_fwd", &pb::attn_fwd);

@@ -1,0 +1,542 @@
+// Batched tcgen05 products of the Newton-Schulz iteration (sm_100a).
+//
+// One step on a matrix X [m, n] is, with r = min(m, n),
+//
+//   A = X X^T (wide, m <= n) or X^T X (tall)      GRAM    r x r, symmetric
+//   P = a I + b A + c A A                         POLY    r x r, symmetric
+//   X <- P X (wide) or X P (tall)                 APPLY / LAST / STEP   m x n
+//
+// A launch does one of these products for every matrix of up to kNsGroups groups; a group is
+// a set of matrices of one shape, stored back to back, so one 3-D tensor map addresses all of
+// them and its bounds zero-fill ragged edges.  X is never transposed: both operands of a
+// tcgen05.mma may be K-major or MN-major, and the group says which.
+//
+// Numbers.  Operands are fp16 (11 significant bits; bf16 iterates lose an order of magnitude
+// against the 64-bit iteration), held at fixed power-of-two scales that keep everything the
+// iteration produces (|X| <= ~1.2, |A| <= ~1.5, |P| <= 3.5 in the 2-norm) in fp16's normal
+// range.  Accumulation is fp32.  Small singular values grow 3.4-fold per step, and with them
+// the rounding of X in the directions X hardly has: so the early iterates carry their
+// rounding error as a second fp16 matrix ``low`` (scaled by 2^11), which enters through the
+// linear term, X' = P hi + a low.  Simulated against 64 bits over Gaussian, low-rank and
+// power-law spectra the result is off by at most 2.9e-3 of its norm (without ``low`` 4e-2).
+//
+// Kernel structure: that of the CTA-pair GEMM (gemm_pair.cuh), whose barrier and abort
+// protocol is kept.  CG = 2: a pair of CTAs computes a 256 x 256 tile with cta_group::2; CG =
+// 1: one CTA computes 128 x 128, for launches too small to fill the GPU with pairs.  Either
+// way a CTA stages 128 rows of each operand per 64-deep k-block (32 KB), loaded as four
+// 64 x 64 boxes.  GRAM and POLY compute the tiles on and above the diagonal only and store
+// each off-diagonal tile twice, once transposed in registers-to-shared staging.
+//   warp 0 TMA producer, warp 1 TMEM allocation and MMA issue, warps 2-5 epilogue.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "gemm_pair.cuh"
+
+namespace pb {
+
+enum NsMode : int {
+  NS_GRAM = 0,   // out = alpha acc
+  NS_POLY = 1,   // out = alpha acc + beta add + diag I
+  NS_APPLY = 2,  // out, low = split(alpha acc + beta add)  (``add``: the input's low part, or none)
+  NS_LAST = 3,   // bf16 result
+  NS_STEP = 4,   // p = decay p - step alpha acc (fp32), and the bf16 copy of p
+};
+
+constexpr int kNsGroups = 8;     // shapes per launch
+constexpr int kNsMats = 192;     // matrices per launch of the pointer tables
+constexpr float kNsLowScale = 2048.f;
+
+struct NsGroup {
+  CUtensorMap a, b;      // operands: 64 x 64 boxes of fp16 [batch][rows][cols]
+  CUtensorMap out, low;  // 32 x 32 boxes of the results
+  const __half* add;     // POLY / APPLY addend, indexed as the result (null: none)
+  long add_batch;        // elements between the addend's matrices
+  int add_ld;
+  int M, N, K;
+  int a_mn, b_mn;        // operand is MN-major
+  int batch;             // matrices
+  int k_blocks;
+  int tiles_n;           // tiles per row (symmetric: per side)
+  int tiles_per_mat;
+  int tile_end;          // running total over the groups
+  int store_low;         // APPLY: the result's low part is wanted
+  int mat0;              // STEP: index of the group's first matrix in the pointer table
+  __nv_bfloat16* dst;    // LAST: [batch][M][N]
+  int dst_tma;           // LAST: ``out`` maps dst (rows are whole 16-byte pieces)
+  float step;            // STEP: step length per unit of learning rate
+};
+struct NsArgs {
+  NsGroup g[kNsGroups];
+  int groups;
+  int tiles;
+  float alpha, beta, diag;
+  int* status;
+};
+struct NsStepArgs {
+  float* p[kNsMats];
+  __nv_bfloat16* shadow[kNsMats];
+  const float* norm;  // gradient norm; not finite: nothing is updated (null: always update)
+  const float* hp;    // learning rate on the device (null: ``lr``)
+  float lr, weight_decay;
+};
+struct NsNoStep {};
+
+template <int CG_>
+struct NsCfg {
+  static constexpr int CG = CG_;
+  static constexpr int BM = 128;
+  static constexpr int T = BM * CG;  // tile rows and columns
+  static constexpr int BK = 64;
+  static constexpr int OP_BYTES = BM * BK * 2;  // this CTA's share of either operand
+  static constexpr int STAGE_BYTES = 2 * OP_BYTES;
+  static constexpr int STAGES = 5;
+  using Stg = StagerT<8>;
+  static constexpr int EPI_OFF = STAGES * STAGE_BYTES;
+  static constexpr uint32_t TMEM_COLS = 2 * T;
+  static constexpr int SMEM_BYTES = EPI_OFF + 4 * Stg::kBytes + 1024;
+  static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+};
+
+// kind::f16 instruction descriptor with fp16 operands (formats 0) and fp32 accumulation.
+__device__ __forceinline__ uint32_t ns_idesc(int t, int a_mn, int b_mn) {
+  return (1u << 4) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) |
+         (static_cast<uint32_t>(t >> 3) << 17) | (static_cast<uint32_t>(t >> 4) << 24);
+}
+
+struct NsTile {
+  int g, mat, i, j;
+};
+// Tile index -> group, matrix and tile row / column (i <= j where only one half is computed).
+__device__ __forceinline__ NsTile ns_tile(const NsArgs& a, int tile, bool sym) {
+  int g = 0, base = 0;
+  while (g + 1 < a.groups && tile >= a.g[g].tile_end) base = a.g[g++].tile_end;
+  const int per = a.g[g].tiles_per_mat, tn = a.g[g].tiles_n;
+  const int local = tile - base;
+  NsTile t{g, local / per, 0, 0};
+  int k = local % per;
+  if (sym) {
+    int len = tn;
+    while (k >= len) {
+      k -= len--;
+      ++t.i;
+    }
+    t.j = t.i + k;
+  } else {
+    t.i = k / tn;
+    t.j = k % tn;
+  }
+  return t;
+}
+
+template <int CG>
+__device__ __forceinline__ void ns_load(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+// 128 rows (K-major) or columns (MN-major) of an operand from ``row``, k-block ``k0``.
+template <int CG>
+__device__ __forceinline__ void ns_load_operand(uint8_t* dst, const CUtensorMap* map, uint32_t bar, int mn, int row,
+                                                int k0, int mat) {
+  if (mn) {
+    ns_load<CG>(dst, map, bar, row, k0, mat);
+    ns_load<CG>(dst + 8192, map, bar, row + 64, k0, mat);
+  } else {
+    ns_load<CG>(dst, map, bar, k0, row, mat);
+    ns_load<CG>(dst + 8192, map, bar, k0, row + 64, mat);
+  }
+}
+
+__device__ __forceinline__ void ns_store(const CUtensorMap* map, const uint8_t* s, int col, int row, int mat) {
+  fence_async_smem();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(s)), "r"(col), "r"(row), "r"(mat)
+                 : "memory");
+    bulk_commit();
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 32 values of this lane's row -> 64-byte row of a 64B-swizzled [32 x 32] fp16 box.
+__device__ __forceinline__ void stage_f16(uint8_t* s, const float (&v)[32]) {
+  const int r = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4 q = make_uint4(pack_f16x2(v[8 * j], v[8 * j + 1]), pack_f16x2(v[8 * j + 2], v[8 * j + 3]),
+                         pack_f16x2(v[8 * j + 4], v[8 * j + 5]), pack_f16x2(v[8 * j + 6], v[8 * j + 7]));
+    *reinterpret_cast<uint4*>(s + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)) = q;
+  }
+}
+// The same box transposed: this lane's 32 values become column ``lane``.
+__device__ __forceinline__ void stage_f16_t(uint8_t* s, const float (&v)[32]) {
+  const int c = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    *reinterpret_cast<__half*>(s + j * 64 + (((c >> 3) ^ ((j >> 1) & 3)) << 4) + (c & 7) * 2) = __float2half_rn(v[j]);
+}
+
+// 32 fp16 of this lane's row of the addend, columns [col, col + 32); pieces at or beyond ``ld``
+// (the padded row length, a multiple of 8) read as zero.
+__device__ __forceinline__ void ns_load_add(const __half* row, bool ok, int col, int ld, uint4 (&q)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    q[j] = ok && col + 8 * j < ld ? __ldg(reinterpret_cast<const uint4*>(row + col) + j) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void ns_add(float (&v)[32], const uint4 (&q)[4], float alpha, float beta) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t* w = &q[j].x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(w + k));
+      v[8 * j + 2 * k] = alpha * v[8 * j + 2 * k] + beta * f.x;
+      v[8 * j + 2 * k + 1] = alpha * v[8 * j + 2 * k + 1] + beta * f.y;
+    }
+  }
+}
+
+// A 32 x 32 fp32 block through shared memory: lane-major in, column-major out, no conflicts.
+__device__ __forceinline__ void ns_transpose_in(float* s, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[lane * 32 + (j ^ lane)] = v[j];
+  __syncwarp();
+}
+
+// Epilogue of one tile for the 32 rows from ``row0``.
+template <int CG, int MODE, class Step>
+__device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, const NsTile& t, typename NsCfg<CG>::Stg& st,
+                                            uint32_t tacc, int row0) {
+  using C = NsCfg<CG>;
+  const NsGroup& g = a.g[t.g];
+  const int lane = threadIdx.x & 31;
+  const int row = row0 + lane;
+  if constexpr (MODE == NS_GRAM || MODE == NS_POLY || MODE == NS_APPLY) {
+    const bool with_add = MODE != NS_GRAM && g.add != nullptr;
+    const bool ok = with_add && row < g.M;
+    const __half* arow = with_add ? g.add + t.mat * g.add_batch + static_cast<long>(ok ? row : 0) * g.add_ld : nullptr;
+    uint4 q[4];
+    if (with_add) ns_load_add(arow, ok, t.j * C::T, g.add_ld, q);
+    tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
+      const int col = t.j * C::T + c;
+      if (col >= g.N) return;  // uniform across the warp
+      if (with_add) {
+        uint4 qn[4];
+        if (c + 32 < C::T) ns_load_add(arow, ok, col + 32, g.add_ld, qn);
+        ns_add(v, q, a.alpha, a.beta);
+        if (c + 32 < C::T) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) q[j] = qn[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= a.alpha;
+      }
+      if constexpr (MODE == NS_POLY) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (col + j == row) v[j] += a.diag;
+      }
+      uint8_t* s = st.acquire();
+      stage_f16(s, v);
+      ns_store(&g.out, s, col, row0, t.mat);
+      st.release();
+      if constexpr (MODE == NS_APPLY) {
+        if (g.store_low) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = (v[j] - __half2float(__float2half_rn(v[j]))) * kNsLowScale;
+          s = st.acquire();
+          stage_f16(s, v);
+          ns_store(&g.low, s, col, row0, t.mat);
+          st.release();
+        }
+      } else if (t.i != t.j && row0 < g.N) {  // the mirrored tile; rows and columns swap
+        s = st.acquire();
+        stage_f16_t(s, v);
+        ns_store(&g.out, s, row0, col, t.mat);
+        st.release();
+      }
+    });
+  } else if constexpr (MODE == NS_LAST) {
+    if (g.dst_tma) {
+      tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
+        const int col = t.j * C::T + c;
+        if (col >= g.N) return;
+        uint8_t* s = st.acquire();
+        stage_bf16(s, v, a.alpha);
+        ns_store(&g.out, s, col, row0, t.mat);
+        st.release();
+      });
+    } else {
+      // rows that do not start on 16-byte boundaries: 64-byte row pieces with plain stores
+      float* s = reinterpret_cast<float*>(st.base);
+      __nv_bfloat16* d = g.dst + static_cast<long>(t.mat) * g.M * g.N;
+      const int rows = min(32, g.M - row0);
+      tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
+        const int col = t.j * C::T + c;
+        if (col >= g.N) return;
+        ns_transpose_in(s, v);
+        if (col + lane < g.N)
+          for (int k = 0; k < rows; ++k)
+            d[static_cast<long>(row0 + k) * g.N + col + lane] = __float2bfloat16_rn(s[k * 32 + (lane ^ k)] * a.alpha);
+        __syncwarp();
+      });
+    }
+  } else {
+    if (sa.norm != nullptr && !isfinite(*sa.norm)) return;
+    const float lr = sa.hp != nullptr ? *sa.hp : sa.lr;
+    const float decay = 1.f - lr * sa.weight_decay;
+    const float step = lr * g.step * a.alpha;
+    float* p = sa.p[g.mat0 + t.mat];
+    __nv_bfloat16* sh = sa.shadow[g.mat0 + t.mat];
+    float* s = reinterpret_cast<float*>(st.base);
+    const int rows = min(32, g.M - row0);
+    float cur[32];
+    auto fetch = [&](int col, float (&w)[32]) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        w[k] = k < rows && col + lane < g.N ? p[static_cast<long>(row0 + k) * g.N + col + lane] : 0.f;
+    };
+    fetch(t.j * C::T, cur);
+    tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
+      const int col = t.j * C::T + c;
+      if (col >= g.N) return;
+      ns_transpose_in(s, v);
+      float next[32];
+      if (c + 32 < C::T) fetch(col + 32, next);
+      if (col + lane < g.N) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          if (k < rows) {
+            const float w = cur[k] * decay - step * s[k * 32 + (lane ^ k)];
+            const long at = static_cast<long>(row0 + k) * g.N + col + lane;
+            p[at] = w;
+            if (sh != nullptr) sh[at] = __float2bfloat16_rn(w);
+          }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 32; ++k) cur[k] = next[k];
+    });
+  }
+}
+
+// 192 threads; CG == 2 with cluster dimension (2, 1, 1).
+template <int CG, int MODE, class Step>
+__global__ void __launch_bounds__(192, 1)
+    ns_gemm_kernel(const __grid_constant__ NsArgs args, const __grid_constant__ Step step) {
+  using C = NsCfg<CG>;
+  constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t accf_bar[2];
+  __shared__ __align__(8) uint64_t acce_bar[2];
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile int abort_sh;
+  __shared__ volatile uint32_t odd_done_sh;  // even CTA: the odd producer's issued k-blocks | kOddDone
+  extern __shared__ uint8_t dyn_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const uint32_t cta = CG == 2 ? cluster_ctarank() : 0;  // CTA 0 issues the MMAs
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+  if (threadIdx.x == 0) {
+    odd_done_sh = 0;
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&accf_bar[s], 1);
+      mbar_init(&acce_bar[s], 4 * CG);
+    }
+    mbar_init(&drain_bar, 1);
+    abort_sh = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(&tmem_base_sh, C::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&tmem_base_sh, C::TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_sh;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t full0 = CG == 2 ? cluster_addr(smem_u32(&full_bar[0]), 0) : smem_u32(&full_bar[0]);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t armed_mask = 0, armed_phase = 0;  // CTA 0: per stage, armed and its phase
+      uint32_t n_kb = 0;                         // k-blocks armed (CTA 0) / issued (CTA 1)
+      bool ok = true;
+      for (int tile = first; tile < args.tiles && ok; tile += stride) {
+        const NsTile t = ns_tile(args, tile, SYM);
+        const NsGroup& g = args.g[t.g];
+        const int row_a = t.i * C::T + static_cast<int>(cta) * C::BM;
+        const int row_b = t.j * C::T + static_cast<int>(cta) * C::BM;
+        const int a_mn = g.a_mn, b_mn = g.b_mn, kbs = g.k_blocks;
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, args.status, 141, &abort_sh)) {
+            ok = false;
+            break;
+          }
+          if (cta == 0) {
+            mbar_arrive_expect_tx(&full_bar[stage], CG * C::STAGE_BYTES);
+            armed_mask |= 1u << stage;
+            armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
+          }
+          ++n_kb;
+          uint8_t* sa = smem + stage * C::STAGE_BYTES;
+          ns_load_operand<CG>(sa, &g.a, full0 + stage * 8, a_mn, row_a, kb * C::BK, t.mat);
+          ns_load_operand<CG>(sa + C::OP_BYTES, &g.b, full0 + stage * 8, b_mn, row_b, kb * C::BK, t.mat);
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // Abort protocol of gemm_pair.cuh: no load of either CTA is in flight at the exit.
+      if (CG == 2 && cta == 1) {
+        st_release_cluster(cluster_addr(smem_u32((const void*)&odd_done_sh), 0), n_kb | kOddDone);
+      } else if (!ok) {
+        if constexpr (CG == 2) {
+          st_release_cluster(cluster_addr(smem_u32((const void*)&abort_sh), 1), 1u);
+          uint32_t done = 0;
+          const uint64_t t0 = globaltimer();
+          while (!((done = ld_acquire_cluster(&odd_done_sh)) & kOddDone)) {
+            if (globaltimer() - t0 > 2 * PB_WAIT_TIMEOUT_NS) {
+              report_error(args.status, 147);
+              break;
+            }
+          }
+          if (done & kOddDone) {
+            const uint32_t n_odd = done & ~kOddDone;
+            for (uint32_t kb = n_kb; kb < n_odd && kb < n_kb + C::STAGES; ++kb) {
+              mbar_arrive_expect_tx(&full_bar[stage], C::STAGE_BYTES);
+              armed_mask |= 1u << stage;
+              armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
+              if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
+          }
+        }
+        for (int s = 0; s < C::STAGES; ++s)
+          if (armed_mask & (1u << s)) mbar_wait(&full_bar[s], (armed_phase >> s) & 1u, args.status, 142, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (cta == 0 && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int tile = first; tile < args.tiles && ok; tile += stride) {
+        const NsGroup& g = args.g[ns_tile(args, tile, SYM).g];
+        const int a_mn = g.a_mn, b_mn = g.b_mn, kbs = g.k_blocks;
+        const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
+        // K-major: 32 bytes per 16-deep step; MN-major: 16 rows of 128 bytes
+        const uint32_t step_a = a_mn ? 2048 : 32, step_b = b_mn ? 2048 : 32;
+        const uint32_t lbo_a = a_mn ? 8192 : 16, lbo_b = b_mn ? 8192 : 16;
+        if (!mbar_wait(&acce_bar[acc], acc_phase ^ 1, args.status, 143, &abort_sh)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * C::T;
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, args.status, 144, &abort_sh)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t s0 = smem_u32(smem + stage * C::STAGE_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < C::BK / 16; ++kk) {
+            const uint64_t ad = sdesc_sw128(s0 + kk * step_a, lbo_a, 1024);
+            const uint64_t bd = sdesc_sw128(s0 + C::OP_BYTES + kk * step_b, lbo_b, 1024);
+            if constexpr (CG == 2) umma_ss_pair(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            else umma_ss(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          }
+          if constexpr (CG == 2) umma_commit_both(&empty_bar[stage]);
+          else umma_commit(&empty_bar[stage]);
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        if constexpr (CG == 2) umma_commit_both(&accf_bar[acc]);
+        else umma_commit(&accf_bar[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+      // All MMAs issued by this thread must finish before TMEM is released.
+      if constexpr (CG == 2) umma_commit_pair_local(&drain_bar);
+      else umma_commit(&drain_bar);
+      mbar_wait(&drain_bar, 0, args.status, 145, nullptr);
+    }
+  } else {
+    const int q = warp & 3;
+    const uint32_t acce0 = CG == 2 ? cluster_addr(smem_u32(&acce_bar[0]), 0) : 0;
+    typename C::Stg st{smem + C::EPI_OFF + q * C::Stg::kBytes, 0, false};
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = first; tile < args.tiles; tile += stride) {
+      const NsTile t = ns_tile(args, tile, SYM);
+      if (!mbar_wait_warp(&accf_bar[acc], acc_phase, args.status, 146, &abort_sh)) break;
+      tc_fence_after();
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::T;
+      const int row0 = t.i * C::T + static_cast<int>(cta) * C::BM + q * 32;
+      if (row0 < args.g[t.g].M) ns_epilogue<CG, MODE>(args, step, t, st, tacc, row0);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(acce0 + acc * 8);
+        else mbar_arrive(&acce_bar[acc]);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_all<0>();
+    __syncwarp();
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+    else tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+}  // namespace pb

@@ -66,6 +66,13 @@ STATUS_NAMES = {
     104: "gemm mma: tile copy never landed",
     105: "gemm mma: drain",
     106: "gemm epilogue: accumulator never ready",
+    141: "newton-schulz producer: smem slot never freed",
+    142: "newton-schulz producer: drain of in-flight copies",
+    143: "newton-schulz mma: accumulator never released",
+    144: "newton-schulz mma: tile copy never landed",
+    145: "newton-schulz mma: drain",
+    146: "newton-schulz epilogue: accumulator never ready",
+    147: "newton-schulz producer: the other CTA's count never came",
 }
 
 

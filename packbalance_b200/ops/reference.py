@@ -21,6 +21,21 @@ def layernorm_reference(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     return (y if bias is None else y + bias.float()).to(x.dtype)
 
 
+def newton_schulz_reference(u: torch.Tensor, steps: int, coefficients: tuple[float, float, float],
+                            eps: float) -> torch.Tensor:
+    """``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` from
+    ``X = u / (|u|_F + eps)``, over the last two dimensions, in ``u``'s type."""
+    a, b, c = coefficients
+    x = u / (u.square().sum(dim=(-2, -1), keepdim=True).sqrt() + eps)
+    tall = x.shape[-2] > x.shape[-1]
+    if tall:
+        x = x.transpose(-2, -1)
+    for _ in range(steps):
+        gram = x @ x.transpose(-2, -1)
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.transpose(-2, -1) if tall else x
+
+
 def swiglu_reference(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return F.silu(gate) * up
 
