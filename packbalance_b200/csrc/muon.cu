@@ -431,7 +431,7 @@ void ns_launch(const NsArgs& args, const Step& step, int dev, cudaStream_t strea
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(192, 1, 1);
+  cfg.blockDim = dim3(C::THREADS, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -449,18 +449,26 @@ void ns_launch(const NsArgs& args, const Step& step, int dev, cudaStream_t strea
   PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, args, step));
 }
 
-// Tile counts of every group for tile side ``T``; returns the total.
-int64_t count_tiles(NsArgs& a, int T, bool sym) {
+// Tile counts of every group; returns the total.
+template <int CG, bool SYM>
+int64_t count_tiles(NsArgs& a) {
+  constexpr int T = NsCfg<CG>::T;
   int64_t total = 0;
   for (int k = 0; k < a.groups; ++k) {
     NsGroup& g = a.g[k];
-    const int64_t tm = (g.M + T - 1) / T, tn = (g.N + T - 1) / T;
-    g.tiles_n = static_cast<int>(tn);
-    g.tiles_per_mat = static_cast<int>(sym ? tn * (tn + 1) / 2 : tm * tn);
-    total += static_cast<int64_t>(g.tiles_per_mat) * g.batch;
+    const int tm = (g.M + T - 1) / T, tn = (g.N + T - 1) / T;
+    int64_t per = static_cast<int64_t>(tm) * tn;
+    if (SYM) {
+      per = 0;
+      for (int i = 0; i < tm; ++i) per += tn - ns_first_col<CG>(i);
+    }
+    TORCH_CHECK(per < (1LL << 31), "newton-schulz: too many tiles");
+    g.tiles_n = tn;
+    g.tiles_per_mat = static_cast<int>(per);
+    total += per * g.batch;
+    TORCH_CHECK(total < (1LL << 31), "newton-schulz: too many tiles");
     g.tile_end = static_cast<int>(total);
   }
-  TORCH_CHECK(total < (1LL << 31), "newton-schulz: too many tiles");
   a.tiles = static_cast<int>(total);
   return total;
 }
@@ -471,10 +479,10 @@ void ns_product(NsArgs& a, const Step& step, int dev, cudaStream_t s) {
   // 256-wide pair tiles once they fill the pairs; below that the smaller tiles spread the
   // work over more SMs.
   const int64_t pairs = num_sms(dev) / 2;
-  if (count_tiles(a, 256, SYM) >= pairs) {
+  if (count_tiles<2, SYM>(a) >= pairs) {
     ns_launch<2, MODE, Step>(a, step, dev, s);
   } else {
-    count_tiles(a, 128, SYM);
+    count_tiles<1, SYM>(a);
     ns_launch<1, MODE, Step>(a, step, dev, s);
   }
 }
@@ -522,6 +530,7 @@ void ns_iterate(std::vector<Shape>& shapes, const Iteration& it, int dev, cudaSt
         q.add = sh.gram;
         q.add_batch = r * sh.ldr();
         q.add_ld = (int)sh.ldr();
+        q.a_sym = q.b_sym = 1;
         q.M = q.N = q.K = (int)r;
         q.k_blocks = (q.K + 63) / 64;
       }
@@ -529,7 +538,8 @@ void ns_iterate(std::vector<Shape>& shapes, const Iteration& it, int dev, cudaSt
       const CUtensorMap p = load_map(sh.poly, r, r, B, sh.ldr());
       y.a = sh.tall() ? x : p;
       y.b = sh.tall() ? p : x;
-      y.a_mn = 0;
+      y.a_sym = !sh.tall();
+      y.b_sym = sh.tall();
       y.b_mn = !sh.tall();
       y.M = (int)sh.rows;
       y.N = (int)sh.cols;
@@ -865,7 +875,13 @@ void muon_update(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, 
     ns_passes<float, true>(pa, t, blocks, s);
     ns_iterate(shapes, it, dev, s, [&](NsArgs& a) {
       for (int j = 0; j < a.groups; ++j)
-        a.g[j].step = step_length(shapes[j]);
+        {
+        NsGroup& g = a.g[j];
+        g.step = step_length(shapes[j]);
+        g.vec = g.N % 4 == 0;
+        for (int i = 0; i < g.batch; ++i)
+          g.vec = g.vec && aligned16(st.p[g.mat0 + i]) && reinterpret_cast<uintptr_t>(st.shadow[g.mat0 + i]) % 8 == 0;
+      }
       ns_product<NS_STEP>(a, st, dev, s);
     });
   }

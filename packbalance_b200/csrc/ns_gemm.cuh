@@ -24,9 +24,12 @@
 // protocol is kept.  CG = 2: a pair of CTAs computes a 256 x 256 tile with cta_group::2; CG =
 // 1: one CTA computes 128 x 128, for launches too small to fill the GPU with pairs.  Either
 // way a CTA stages 128 rows of each operand per 64-deep k-block (32 KB), loaded as four
-// 64 x 64 boxes.  GRAM and POLY compute the tiles on and above the diagonal only and store
-// each off-diagonal tile twice, once transposed in registers-to-shared staging.
-//   warp 0 TMA producer, warp 1 TMEM allocation and MMA issue, warps 2-5 epilogue.
+// 64 x 64 boxes.  GRAM and POLY compute and store only the 256 x 256 blocks on and above the
+// diagonal.  Whoever reads such a matrix takes a block below the diagonal from its mirror
+// image: the same box load with the coordinates swapped, and that k-block's MMAs told that
+// the operand is MN-major.  So symmetry halves the stores as well as the products.
+//   warp 0 TMA producer, warp 1 TMEM allocation and MMA issue, warps 2-9 epilogue: two per
+//   quarter of the TMEM lanes, each finishing half of the tile's columns.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -55,12 +58,14 @@ struct NsGroup {
   int add_ld;
   int M, N, K;
   int a_mn, b_mn;        // operand is MN-major
+  int a_sym, b_sym;      // operand is symmetric, blocks on and above the diagonal stored
   int batch;             // matrices
   int k_blocks;
   int tiles_n;           // tiles per row (symmetric: per side)
   int tiles_per_mat;
   int tile_end;          // running total over the groups
   int store_low;         // APPLY: the result's low part is wanted
+  int vec;               // STEP: 16-byte accesses to the parameters
   int mat0;              // STEP: index of the group's first matrix in the pointer table
   __nv_bfloat16* dst;    // LAST: [batch][M][N]
   int dst_tma;           // LAST: ``out`` maps dst (rows are whole 16-byte pieces)
@@ -91,10 +96,12 @@ struct NsCfg {
   static constexpr int OP_BYTES = BM * BK * 2;  // this CTA's share of either operand
   static constexpr int STAGE_BYTES = 2 * OP_BYTES;
   static constexpr int STAGES = 5;
-  using Stg = StagerT<8>;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  using Stg = StagerT<4>;
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES;
   static constexpr uint32_t TMEM_COLS = 2 * T;
-  static constexpr int SMEM_BYTES = EPI_OFF + 4 * Stg::kBytes + 1024;
+  static constexpr int SMEM_BYTES = EPI_OFF + EPI_WARPS * Stg::kBytes + 1024;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
@@ -107,26 +114,33 @@ __device__ __forceinline__ uint32_t ns_idesc(int t, int a_mn, int b_mn) {
 struct NsTile {
   int g, mat, i, j;
 };
-// Tile index -> group, matrix and tile row / column (i <= j where only one half is computed).
-__device__ __forceinline__ NsTile ns_tile(const NsArgs& a, int tile, bool sym) {
+// First tile column that is computed in tile row ``i`` of a symmetric result: 256 x 256 blocks
+// are whole, so with 128-wide tiles the block's first.
+template <int CG>
+__host__ __device__ __forceinline__ int ns_first_col(int i) {
+  return CG == 2 ? i : i & ~1;
+}
+// Tile index -> group, matrix and tile row / column.
+template <int CG, bool SYM>
+__device__ __forceinline__ NsTile ns_tile(const NsArgs& a, int tile) {
   int g = 0, base = 0;
   while (g + 1 < a.groups && tile >= a.g[g].tile_end) base = a.g[g++].tile_end;
   const int per = a.g[g].tiles_per_mat, tn = a.g[g].tiles_n;
   const int local = tile - base;
   NsTile t{g, local / per, 0, 0};
   int k = local % per;
-  if (sym) {
-    int len = tn;
-    while (k >= len) {
-      k -= len--;
-      ++t.i;
-    }
-    t.j = t.i + k;
+  if (SYM) {
+    while (k >= tn - ns_first_col<CG>(t.i)) k -= tn - ns_first_col<CG>(t.i++);
+    t.j = ns_first_col<CG>(t.i) + k;
   } else {
     t.i = k / tn;
     t.j = k % tn;
   }
   return t;
+}
+// Is the operand MN-major in k-block ``kb`` of a tile whose rows start at ``row``?
+__device__ __forceinline__ int ns_is_mn(int mn, int sym, int row, int kb) {
+  return sym ? (kb * 64) / 256 < row / 256 : mn;
 }
 
 template <int CG>
@@ -185,14 +199,6 @@ __device__ __forceinline__ void stage_f16(uint8_t* s, const float (&v)[32]) {
     *reinterpret_cast<uint4*>(s + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)) = q;
   }
 }
-// The same box transposed: this lane's 32 values become column ``lane``.
-__device__ __forceinline__ void stage_f16_t(uint8_t* s, const float (&v)[32]) {
-  const int c = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    *reinterpret_cast<__half*>(s + j * 64 + (((c >> 3) ^ ((j >> 1) & 3)) << 4) + (c & 7) * 2) = __float2half_rn(v[j]);
-}
-
 // 32 fp16 of this lane's row of the addend, columns [col, col + 32); pieces at or beyond ``ld``
 // (the padded row length, a multiple of 8) read as zero.
 __device__ __forceinline__ void ns_load_add(const __half* row, bool ok, int col, int ld, uint4 (&q)[4]) {
@@ -213,36 +219,48 @@ __device__ __forceinline__ void ns_add(float (&v)[32], const uint4 (&q)[4], floa
   }
 }
 
-// A 32 x 32 fp32 block through shared memory: lane-major in, column-major out, no conflicts.
-__device__ __forceinline__ void ns_transpose_in(float* s, const float (&v)[32]) {
-  const int lane = threadIdx.x & 31;
+// A 32 x 32 fp32 block through shared memory: this lane's row in, any row's 16-byte pieces out
+// (piece q of row r at q ^ (r & 7): neither direction has bank conflicts).
+__device__ __forceinline__ void ns_block_in(float* s, const float (&v)[32]) {
+  const int r = threadIdx.x & 31;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) s[lane * 32 + (j ^ lane)] = v[j];
+  for (int q = 0; q < 8; ++q)
+    *reinterpret_cast<float4*>(s + r * 32 + ((q ^ (r & 7)) << 2)) =
+        make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
   __syncwarp();
 }
+__device__ __forceinline__ float4 ns_block_piece(const float* s, int r, int q) {
+  return *reinterpret_cast<const float4*>(s + r * 32 + ((q ^ (r & 7)) << 2));
+}
+__device__ __forceinline__ float ns_block_at(const float* s, int r, int c) {
+  return s[r * 32 + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3))];
+}
 
-// Epilogue of one tile for the 32 rows from ``row0``.
+// Epilogue of one tile for the 32 rows from ``row0`` and the tile columns [c0, c0 + T / 2);
+// ``tacc`` is the accumulator's address at those rows and columns.
 template <int CG, int MODE, class Step>
 __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, const NsTile& t, typename NsCfg<CG>::Stg& st,
-                                            uint32_t tacc, int row0) {
+                                            uint32_t tacc, int row0, int c0) {
   using C = NsCfg<CG>;
+  constexpr int W = C::T / 2;
   const NsGroup& g = a.g[t.g];
   const int lane = threadIdx.x & 31;
   const int row = row0 + lane;
+  const int col0 = t.j * C::T + c0;
   if constexpr (MODE == NS_GRAM || MODE == NS_POLY || MODE == NS_APPLY) {
     const bool with_add = MODE != NS_GRAM && g.add != nullptr;
     const bool ok = with_add && row < g.M;
     const __half* arow = with_add ? g.add + t.mat * g.add_batch + static_cast<long>(ok ? row : 0) * g.add_ld : nullptr;
     uint4 q[4];
-    if (with_add) ns_load_add(arow, ok, t.j * C::T, g.add_ld, q);
-    tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
-      const int col = t.j * C::T + c;
+    if (with_add) ns_load_add(arow, ok, col0, g.add_ld, q);
+    tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
+      const int col = col0 + c;
       if (col >= g.N) return;  // uniform across the warp
       if (with_add) {
         uint4 qn[4];
-        if (c + 32 < C::T) ns_load_add(arow, ok, col + 32, g.add_ld, qn);
+        if (c + 32 < W) ns_load_add(arow, ok, col + 32, g.add_ld, qn);
         ns_add(v, q, a.alpha, a.beta);
-        if (c + 32 < C::T) {
+        if (c + 32 < W) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) q[j] = qn[j];
         }
@@ -251,9 +269,11 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
         for (int j = 0; j < 32; ++j) v[j] *= a.alpha;
       }
       if constexpr (MODE == NS_POLY) {
+        if (col < row0 + 32 && row0 < col + 32) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col + j == row) v[j] += a.diag;
+          for (int j = 0; j < 32; ++j)
+            if (col + j == row) v[j] += a.diag;
+        }
       }
       uint8_t* s = st.acquire();
       stage_f16(s, v);
@@ -268,17 +288,12 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
           ns_store(&g.low, s, col, row0, t.mat);
           st.release();
         }
-      } else if (t.i != t.j && row0 < g.N) {  // the mirrored tile; rows and columns swap
-        s = st.acquire();
-        stage_f16_t(s, v);
-        ns_store(&g.out, s, row0, col, t.mat);
-        st.release();
       }
     });
   } else if constexpr (MODE == NS_LAST) {
     if (g.dst_tma) {
-      tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
-        const int col = t.j * C::T + c;
+      tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
+        const int col = col0 + c;
         if (col >= g.N) return;
         uint8_t* s = st.acquire();
         stage_bf16(s, v, a.alpha);
@@ -290,17 +305,19 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
       float* s = reinterpret_cast<float*>(st.base);
       __nv_bfloat16* d = g.dst + static_cast<long>(t.mat) * g.M * g.N;
       const int rows = min(32, g.M - row0);
-      tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
-        const int col = t.j * C::T + c;
+      tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
+        const int col = col0 + c;
         if (col >= g.N) return;
-        ns_transpose_in(s, v);
+        ns_block_in(s, v);
         if (col + lane < g.N)
           for (int k = 0; k < rows; ++k)
-            d[static_cast<long>(row0 + k) * g.N + col + lane] = __float2bfloat16_rn(s[k * 32 + (lane ^ k)] * a.alpha);
+            d[static_cast<long>(row0 + k) * g.N + col + lane] = __float2bfloat16_rn(ns_block_at(s, k, lane) * a.alpha);
         __syncwarp();
       });
     }
   } else {
+    // The parameters of the next 32 columns are on their way while this block is updated: the
+    // launch reads and writes 4 bytes per element, more than its products cost.
     if (sa.norm != nullptr && !isfinite(*sa.norm)) return;
     const float lr = sa.hp != nullptr ? *sa.hp : sa.lr;
     const float decay = 1.f - lr * sa.weight_decay;
@@ -308,41 +325,70 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
     float* p = sa.p[g.mat0 + t.mat];
     __nv_bfloat16* sh = sa.shadow[g.mat0 + t.mat];
     float* s = reinterpret_cast<float*>(st.base);
-    const int rows = min(32, g.M - row0);
-    float cur[32];
-    auto fetch = [&](int col, float (&w)[32]) {
+    if (g.vec) {
+      // a lane takes the 16-byte piece lane % 8 of rows lane / 8, + 4, + 8, ...
+      const int r0 = lane >> 3, q = lane & 7;
+      float4 cur[8], next[8];
+      auto fetch = [&](int col, float4 (&w)[8]) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k)
-        w[k] = k < rows && col + lane < g.N ? p[static_cast<long>(row0 + k) * g.N + col + lane] : 0.f;
-    };
-    fetch(t.j * C::T, cur);
-    tmem_walk(tacc, C::T, [&](int c, float (&v)[32]) {
-      const int col = t.j * C::T + c;
-      if (col >= g.N) return;
-      ns_transpose_in(s, v);
-      float next[32];
-      if (c + 32 < C::T) fetch(col + 32, next);
-      if (col + lane < g.N) {
+        for (int k = 0; k < 8; ++k)
+          w[k] = row0 + r0 + 4 * k < g.M && col + 4 * q < g.N
+                     ? *reinterpret_cast<const float4*>(p + static_cast<long>(row0 + r0 + 4 * k) * g.N + col + 4 * q)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      fetch(col0, cur);
+      tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
+        const int col = col0 + c;
+        if (col >= g.N) return;
+        ns_block_in(s, v);
+        if (c + 32 < W) fetch(col + 32, next);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = r0 + 4 * k;
+          const float4 o = ns_block_piece(s, r, q);
+          float4 w = cur[k];
+          w.x = w.x * decay - step * o.x;
+          w.y = w.y * decay - step * o.y;
+          w.z = w.z * decay - step * o.z;
+          w.w = w.w * decay - step * o.w;
+          if (row0 + r < g.M && col + 4 * q < g.N) {
+            const long at = static_cast<long>(row0 + r) * g.N + col + 4 * q;
+            *reinterpret_cast<float4*>(p + at) = w;
+            if (sh != nullptr)
+              *reinterpret_cast<uint2*>(sh + at) = make_uint2(pack_bf16x2(w.x, w.y), pack_bf16x2(w.z, w.w));
+          }
+          cur[k] = next[k];
+        }
+        __syncwarp();
+      });
+    } else {
+      const int rows = min(32, g.M - row0);
+      tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
+        const int col = col0 + c;
+        if (col >= g.N) return;
+        ns_block_in(s, v);
+        float w[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          w[k] = k < rows && col + lane < g.N ? p[static_cast<long>(row0 + k) * g.N + col + lane] : 0.f;
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          if (k < rows) {
-            const float w = cur[k] * decay - step * s[k * 32 + (lane ^ k)];
+          if (k < rows && col + lane < g.N) {
+            const float u = w[k] * decay - step * ns_block_at(s, k, lane);
             const long at = static_cast<long>(row0 + k) * g.N + col + lane;
-            p[at] = w;
-            if (sh != nullptr) sh[at] = __float2bfloat16_rn(w);
+            p[at] = u;
+            if (sh != nullptr) sh[at] = __float2bfloat16_rn(u);
           }
         }
-      }
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k < 32; ++k) cur[k] = next[k];
-    });
+        __syncwarp();
+      });
+    }
   }
 }
 
-// 192 threads; CG == 2 with cluster dimension (2, 1, 1).
+// NsCfg::THREADS threads; CG == 2 with cluster dimension (2, 1, 1).
 template <int CG, int MODE, class Step>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
     ns_gemm_kernel(const __grid_constant__ NsArgs args, const __grid_constant__ Step step) {
   using C = NsCfg<CG>;
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
@@ -369,7 +415,7 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&accf_bar[s], 1);
-      mbar_init(&acce_bar[s], 4 * CG);
+      mbar_init(&acce_bar[s], C::EPI_WARPS * CG);
     }
     mbar_init(&drain_bar, 1);
     abort_sh = 0;
@@ -399,11 +445,11 @@ __global__ void __launch_bounds__(192, 1)
       uint32_t n_kb = 0;                         // k-blocks armed (CTA 0) / issued (CTA 1)
       bool ok = true;
       for (int tile = first; tile < args.tiles && ok; tile += stride) {
-        const NsTile t = ns_tile(args, tile, SYM);
+        const NsTile t = ns_tile<CG, SYM>(args, tile);
         const NsGroup& g = args.g[t.g];
         const int row_a = t.i * C::T + static_cast<int>(cta) * C::BM;
         const int row_b = t.j * C::T + static_cast<int>(cta) * C::BM;
-        const int a_mn = g.a_mn, b_mn = g.b_mn, kbs = g.k_blocks;
+        const int a_mn = g.a_mn, b_mn = g.b_mn, a_sym = g.a_sym, b_sym = g.b_sym, kbs = g.k_blocks;
         for (int kb = 0; kb < kbs; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, args.status, 141, &abort_sh)) {
             ok = false;
@@ -416,8 +462,9 @@ __global__ void __launch_bounds__(192, 1)
           }
           ++n_kb;
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
-          ns_load_operand<CG>(sa, &g.a, full0 + stage * 8, a_mn, row_a, kb * C::BK, t.mat);
-          ns_load_operand<CG>(sa + C::OP_BYTES, &g.b, full0 + stage * 8, b_mn, row_b, kb * C::BK, t.mat);
+          ns_load_operand<CG>(sa, &g.a, full0 + stage * 8, ns_is_mn(a_mn, a_sym, row_a, kb), row_a, kb * C::BK, t.mat);
+          ns_load_operand<CG>(sa + C::OP_BYTES, &g.b, full0 + stage * 8, ns_is_mn(b_mn, b_sym, row_b, kb), row_b,
+                              kb * C::BK, t.mat);
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1;
@@ -463,12 +510,9 @@ __global__ void __launch_bounds__(192, 1)
       uint32_t acc_phase = 0;
       bool ok = true;
       for (int tile = first; tile < args.tiles && ok; tile += stride) {
-        const NsGroup& g = args.g[ns_tile(args, tile, SYM).g];
-        const int a_mn = g.a_mn, b_mn = g.b_mn, kbs = g.k_blocks;
-        const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
-        // K-major: 32 bytes per 16-deep step; MN-major: 16 rows of 128 bytes
-        const uint32_t step_a = a_mn ? 2048 : 32, step_b = b_mn ? 2048 : 32;
-        const uint32_t lbo_a = a_mn ? 8192 : 16, lbo_b = b_mn ? 8192 : 16;
+        const NsTile t = ns_tile<CG, SYM>(args, tile);
+        const NsGroup& g = args.g[t.g];
+        const int kbs = g.k_blocks;
         if (!mbar_wait(&acce_bar[acc], acc_phase ^ 1, args.status, 143, &abort_sh)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * C::T;
@@ -479,6 +523,11 @@ __global__ void __launch_bounds__(192, 1)
           }
           tc_fence_after();
           const uint32_t s0 = smem_u32(smem + stage * C::STAGE_BYTES);
+          const int a_mn = ns_is_mn(g.a_mn, g.a_sym, t.i * C::T, kb), b_mn = ns_is_mn(g.b_mn, g.b_sym, t.j * C::T, kb);
+          const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
+          // K-major: 32 bytes per 16-deep step; MN-major: 16 rows of 128 bytes
+          const uint32_t step_a = a_mn ? 2048 : 32, step_b = b_mn ? 2048 : 32;
+          const uint32_t lbo_a = a_mn ? 8192 : 16, lbo_b = b_mn ? 8192 : 16;
 #pragma unroll
           for (int kk = 0; kk < C::BK / 16; ++kk) {
             const uint64_t ad = sdesc_sw128(s0 + kk * step_a, lbo_a, 1024);
@@ -505,18 +554,19 @@ __global__ void __launch_bounds__(192, 1)
       mbar_wait(&drain_bar, 0, args.status, 145, nullptr);
     }
   } else {
-    const int q = warp & 3;
+    const int q = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 q.., columns T / 2 half..
     const uint32_t acce0 = CG == 2 ? cluster_addr(smem_u32(&acce_bar[0]), 0) : 0;
-    typename C::Stg st{smem + C::EPI_OFF + q * C::Stg::kBytes, 0, false};
+    typename C::Stg st{smem + C::EPI_OFF + (warp - 2) * C::Stg::kBytes, 0, false};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int tile = first; tile < args.tiles; tile += stride) {
-      const NsTile t = ns_tile(args, tile, SYM);
+      const NsTile t = ns_tile<CG, SYM>(args, tile);
       if (!mbar_wait_warp(&accf_bar[acc], acc_phase, args.status, 146, &abort_sh)) break;
       tc_fence_after();
-      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::T;
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::T + half * (C::T / 2);
       const int row0 = t.i * C::T + static_cast<int>(cta) * C::BM + q * 32;
-      if (row0 < args.g[t.g].M) ns_epilogue<CG, MODE>(args, step, t, st, tacc, row0);
+      if (row0 < args.g[t.g].M && t.j * C::T + half * (C::T / 2) < args.g[t.g].N)
+        ns_epilogue<CG, MODE>(args, step, t, st, tacc, row0, half * (C::T / 2));
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
