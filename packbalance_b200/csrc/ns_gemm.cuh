@@ -163,13 +163,9 @@ __device__ __forceinline__ void ns_load(void* dst, const CUtensorMap* map, uint3
 template <int CG>
 __device__ __forceinline__ void ns_load_operand(uint8_t* dst, const CUtensorMap* map, uint32_t bar, int mn, int row,
                                                 int k0, int mat) {
-  if (mn) {
-    ns_load<CG>(dst, map, bar, row, k0, mat);
-    ns_load<CG>(dst + 8192, map, bar, row + 64, k0, mat);
-  } else {
-    ns_load<CG>(dst, map, bar, k0, row, mat);
-    ns_load<CG>(dst + 8192, map, bar, k0, row + 64, mat);
-  }
+  const int x = mn ? row : k0, y = mn ? k0 : row;
+  ns_load<CG>(dst, map, bar, x, y, mat);
+  ns_load<CG>(dst + 8192, map, bar, mn ? x + 64 : x, mn ? y : y + 64, mat);
 }
 
 __device__ __forceinline__ void ns_store(const CUtensorMap* map, const uint8_t* s, int col, int row, int mat) {
@@ -337,11 +333,16 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
                      : make_float4(0.f, 0.f, 0.f, 0.f);
       };
       fetch(col0, cur);
-      tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
+#pragma unroll 1
+      for (int c = 0; c < W; c += 32) {
         const int col = col0 + c;
-        if (col >= g.N) return;
-        ns_block_in(s, v);
+        if (col >= g.N) break;  // uniform across the warp
         if (c + 32 < W) fetch(col + 32, next);
+        {
+          float v[32];
+          tmem_load_f32(tacc + c, v);
+          ns_block_in(s, v);
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int r = r0 + 4 * k;
@@ -360,7 +361,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
           cur[k] = next[k];
         }
         __syncwarp();
-      });
+      }
     } else {
       const int rows = min(32, g.M - row0);
       tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
@@ -509,10 +510,13 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
+      const uint32_t smem_base = smem_u32(smem);
+      const uint64_t desc_k = sdesc_sw128(0, 16, 1024), desc_mn = sdesc_sw128(0, 8192, 1024);
       for (int tile = first; tile < args.tiles && ok; tile += stride) {
         const NsTile t = ns_tile<CG, SYM>(args, tile);
         const NsGroup& g = args.g[t.g];
-        const int kbs = g.k_blocks;
+        const int kbs = g.k_blocks, g_amn = g.a_mn, g_asym = g.a_sym, g_bmn = g.b_mn, g_bsym = g.b_sym;
+        const int row_a = t.i * C::T, row_b = t.j * C::T;
         if (!mbar_wait(&acce_bar[acc], acc_phase ^ 1, args.status, 143, &abort_sh)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * C::T;
@@ -522,18 +526,20 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t s0 = smem_u32(smem + stage * C::STAGE_BYTES);
-          const int a_mn = ns_is_mn(g.a_mn, g.a_sym, t.i * C::T, kb), b_mn = ns_is_mn(g.b_mn, g.b_sym, t.j * C::T, kb);
+          // one thread issues everything, so per MMA there are two additions: 32 bytes per
+          // 16-deep step of a K-major operand, 16 rows of 128 bytes of an MN-major one
+          const uint32_t s0 = smem_base + stage * C::STAGE_BYTES;
+          const bool a_mn = ns_is_mn(g_amn, g_asym, row_a, kb), b_mn = ns_is_mn(g_bmn, g_bsym, row_b, kb);
           const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
-          // K-major: 32 bytes per 16-deep step; MN-major: 16 rows of 128 bytes
-          const uint32_t step_a = a_mn ? 2048 : 32, step_b = b_mn ? 2048 : 32;
-          const uint32_t lbo_a = a_mn ? 8192 : 16, lbo_b = b_mn ? 8192 : 16;
+          uint64_t ad = (a_mn ? desc_mn : desc_k) | (s0 >> 4);
+          uint64_t bd = (b_mn ? desc_mn : desc_k) | ((s0 + C::OP_BYTES) >> 4);
+          const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
           for (int kk = 0; kk < C::BK / 16; ++kk) {
-            const uint64_t ad = sdesc_sw128(s0 + kk * step_a, lbo_a, 1024);
-            const uint64_t bd = sdesc_sw128(s0 + C::OP_BYTES + kk * step_b, lbo_b, 1024);
             if constexpr (CG == 2) umma_ss_pair(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
             else umma_ss(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            ad += step_a;
+            bd += step_b;
           }
           if constexpr (CG == 2) umma_commit_both(&empty_bar[stage]);
           else umma_commit(&empty_bar[stage]);
