@@ -476,14 +476,17 @@ int64_t count_tiles(NsArgs& a) {
 template <int MODE, class Step>
 void ns_product(NsArgs& a, const Step& step, int dev, cudaStream_t s) {
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-  // 256-wide pair tiles once they fill the pairs; below that the smaller tiles spread the
-  // work over more SMs.
-  const int64_t pairs = num_sms(dev) / 2;
-  if (count_tiles<2, SYM>(a) >= pairs) {
-    ns_launch<2, MODE, Step>(a, step, dev, s);
-  } else {
-    count_tiles<1, SYM>(a);
+  // A 256-wide tile on a CTA pair and a 128-wide tile on one CTA take the same time (the pair's
+  // tensor cores finish a k-block in the time in which one CTA's 32 KB of operands arrive), so
+  // the smaller number of waves wins, and at equal numbers the smaller tiles, whose epilogue is
+  // half as long.
+  const int64_t sms = num_sms(dev), pairs = sms / 2;
+  const int64_t waves2 = (count_tiles<2, SYM>(a) + pairs - 1) / pairs, waves1 = (count_tiles<1, SYM>(a) + sms - 1) / sms;
+  if (waves1 <= waves2) {
     ns_launch<1, MODE, Step>(a, step, dev, s);
+  } else {
+    count_tiles<2, SYM>(a);
+    ns_launch<2, MODE, Step>(a, step, dev, s);
   }
 }
 

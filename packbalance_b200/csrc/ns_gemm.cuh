@@ -93,12 +93,12 @@ struct NsCfg {
   static constexpr int BM = 128;
   static constexpr int T = BM * CG;  // tile rows and columns
   static constexpr int BK = 64;
-  static constexpr int OP_BYTES = BM * BK * 2;  // this CTA's share of either operand
+  static constexpr int OP_BYTES = BM * BK * 2;  // this CTA's share of either operand of a k-block
   static constexpr int STAGE_BYTES = 2 * OP_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = 6;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  using Stg = StagerT<4>;
+  using Stg = StagerT<2>;
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES;
   static constexpr uint32_t TMEM_COLS = 2 * T;
   static constexpr int SMEM_BYTES = EPI_OFF + EPI_WARPS * Stg::kBytes + 1024;
@@ -166,6 +166,23 @@ __device__ __forceinline__ void ns_load_operand(uint8_t* dst, const CUtensorMap*
   const int x = mn ? row : k0, y = mn ? k0 : row;
   ns_load<CG>(dst, map, bar, x, y, mat);
   ns_load<CG>(dst + 8192, map, bar, mn ? x + 64 : x, mn ? y : y + 64, mat);
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+// Bounded wait of a whole, converged warp: all lanes try at once, and only if that fails does
+// lane 0 go on polling for the others.
+__device__ __forceinline__ bool ns_wait(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* abort) {
+  if (__all_sync(0xffffffff, mbar_try_wait(bar, parity))) return true;
+  return mbar_wait_warp(bar, parity, status, code, abort);
 }
 
 __device__ __forceinline__ void ns_store(const CUtensorMap* map, const uint8_t* s, int col, int row, int mat) {
@@ -368,17 +385,21 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
         const int col = col0 + c;
         if (col >= g.N) return;
         ns_block_in(s, v);
-        float w[32];
+        if (col + lane < g.N) {
+#pragma unroll 1
+          for (int k0 = 0; k0 < rows; k0 += 8) {
+            float w[8];
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-          w[k] = k < rows && col + lane < g.N ? p[static_cast<long>(row0 + k) * g.N + col + lane] : 0.f;
+            for (int k = 0; k < 8; ++k)
+              w[k] = k0 + k < rows ? p[static_cast<long>(row0 + k0 + k) * g.N + col + lane] : 0.f;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          if (k < rows && col + lane < g.N) {
-            const float u = w[k] * decay - step * ns_block_at(s, k, lane);
-            const long at = static_cast<long>(row0 + k) * g.N + col + lane;
-            p[at] = u;
-            if (sh != nullptr) sh[at] = __float2bfloat16_rn(u);
+            for (int k = 0; k < 8; ++k) {
+              if (k0 + k >= rows) break;
+              const float u = w[k] * decay - step * ns_block_at(s, k0 + k, lane);
+              const long at = static_cast<long>(row0 + k0 + k) * g.N + col + lane;
+              p[at] = u;
+              if (sh != nullptr) sh[at] = __float2bfloat16_rn(u);
+            }
           }
         }
         __syncwarp();
@@ -401,6 +422,7 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_sh;
   __shared__ volatile uint32_t odd_done_sh;  // even CTA: the odd producer's issued k-blocks | kOddDone
+  __shared__ volatile uint32_t odd_one_sh;   // and its one_mask
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
 
@@ -409,7 +431,7 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
   const uint32_t cta = CG == 2 ? cluster_ctarank() : 0;  // CTA 0 issues the MMAs
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
   if (threadIdx.x == 0) {
-    odd_done_sh = 0;
+    odd_done_sh = odd_one_sh = 0;
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
@@ -437,43 +459,56 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
 
+  // Warps 0 and 1 run their loops with all lanes converged and elect one to issue.  A k-block's
+  // MMAs take 512 cycles; measured per k-block the issuing warp spends about 190 on its barrier,
+  // 290 on the four MMAs and 90 on the commit, the producer 360 on four box loads.  A tile on
+  // the diagonal of a symmetric product has twice the same operand and loads it once.
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t full0 = CG == 2 ? cluster_addr(smem_u32(&full_bar[0]), 0) : smem_u32(&full_bar[0]);
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t armed_mask = 0, armed_phase = 0;  // CTA 0: per stage, armed and its phase
-      uint32_t n_kb = 0;                         // k-blocks armed (CTA 0) / issued (CTA 1)
-      bool ok = true;
-      for (int tile = first; tile < args.tiles && ok; tile += stride) {
-        const NsTile t = ns_tile<CG, SYM>(args, tile);
-        const NsGroup& g = args.g[t.g];
-        const int row_a = t.i * C::T + static_cast<int>(cta) * C::BM;
-        const int row_b = t.j * C::T + static_cast<int>(cta) * C::BM;
-        const int a_mn = g.a_mn, b_mn = g.b_mn, a_sym = g.a_sym, b_sym = g.b_sym, kbs = g.k_blocks;
-        for (int kb = 0; kb < kbs; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, args.status, 141, &abort_sh)) {
-            ok = false;
-            break;
-          }
-          if (cta == 0) {
-            mbar_arrive_expect_tx(&full_bar[stage], CG * C::STAGE_BYTES);
-            armed_mask |= 1u << stage;
-            armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
-          }
-          ++n_kb;
-          uint8_t* sa = smem + stage * C::STAGE_BYTES;
+    const uint32_t full0 = CG == 2 ? cluster_addr(smem_u32(&full_bar[0]), 0) : smem_u32(&full_bar[0]);
+    const bool leader = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t armed_mask = 0, armed_phase = 0;  // CTA 0: per stage, armed and its phase
+    uint32_t n_kb = 0;                         // k-blocks armed (CTA 0) / issued (CTA 1)
+    uint32_t one_mask = 0;                     // per stage: its last k-block has one operand
+    bool ok = true;
+    for (int tile = first; tile < args.tiles && ok; tile += stride) {
+      const NsTile t = ns_tile<CG, SYM>(args, tile);
+      const NsGroup& g = args.g[t.g];
+      const int row_a = t.i * C::T + static_cast<int>(cta) * C::BM;
+      const int row_b = t.j * C::T + static_cast<int>(cta) * C::BM;
+      const int a_mn = g.a_mn, b_mn = g.b_mn, a_sym = g.a_sym, b_sym = g.b_sym, kbs = g.k_blocks;
+      const bool one = SYM && t.i == t.j;  // both operands are the same rows of the same matrix
+      for (int kb = 0; kb < kbs; ++kb) {
+        if (!ns_wait(&empty_bar[stage], phase ^ 1, args.status, 141, &abort_sh)) {
+          ok = false;
+          break;
+        }
+        if (cta == 0) {
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * (one ? C::OP_BYTES : C::STAGE_BYTES));
+          armed_mask |= 1u << stage;
+          armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
+        }
+        one_mask = (one_mask & ~(1u << stage)) | (static_cast<uint32_t>(one) << stage);
+        ++n_kb;
+        uint8_t* sa = smem + stage * C::STAGE_BYTES;
+        if (leader) {
           ns_load_operand<CG>(sa, &g.a, full0 + stage * 8, ns_is_mn(a_mn, a_sym, row_a, kb), row_a, kb * C::BK, t.mat);
-          ns_load_operand<CG>(sa + C::OP_BYTES, &g.b, full0 + stage * 8, ns_is_mn(b_mn, b_sym, row_b, kb), row_b,
-                              kb * C::BK, t.mat);
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (!one)
+            ns_load_operand<CG>(sa + C::OP_BYTES, &g.b, full0 + stage * 8, ns_is_mn(b_mn, b_sym, row_b, kb), row_b,
+                                kb * C::BK, t.mat);
+        }
+        __syncwarp();
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
         }
       }
+    }
+    if (leader) {
       // Abort protocol of gemm_pair.cuh: no load of either CTA is in flight at the exit.
       if (CG == 2 && cta == 1) {
+        st_release_cluster(cluster_addr(smem_u32((const void*)&odd_one_sh), 0), one_mask);
         st_release_cluster(cluster_addr(smem_u32((const void*)&odd_done_sh), 0), n_kb | kOddDone);
       } else if (!ok) {
         if constexpr (CG == 2) {
@@ -489,7 +524,7 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
           if (done & kOddDone) {
             const uint32_t n_odd = done & ~kOddDone;
             for (uint32_t kb = n_kb; kb < n_odd && kb < n_kb + C::STAGES; ++kb) {
-              mbar_arrive_expect_tx(&full_bar[stage], C::STAGE_BYTES);
+              mbar_arrive_expect_tx(&full_bar[stage], (odd_one_sh >> stage) & 1u ? C::OP_BYTES : C::STAGE_BYTES);
               armed_mask |= 1u << stage;
               armed_phase = (armed_phase & ~(1u << stage)) | (phase << stage);
               if (++stage == C::STAGES) {
@@ -504,7 +539,8 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (cta == 0 && lane == 0) {
+    if (cta == 0) {
+      const bool leader = elect_one();
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -517,47 +553,56 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
         const NsGroup& g = args.g[t.g];
         const int kbs = g.k_blocks, g_amn = g.a_mn, g_asym = g.a_sym, g_bmn = g.b_mn, g_bsym = g.b_sym;
         const int row_a = t.i * C::T, row_b = t.j * C::T;
-        if (!mbar_wait(&acce_bar[acc], acc_phase ^ 1, args.status, 143, &abort_sh)) break;
+        const bool one = SYM && t.i == t.j;
+        if (!mbar_wait_warp(&acce_bar[acc], acc_phase ^ 1, args.status, 143, &abort_sh)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * C::T;
         for (int kb = 0; kb < kbs; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, args.status, 144, &abort_sh)) {
+          if (!ns_wait(&full_bar[stage], phase, args.status, 144, &abort_sh)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          // one thread issues everything, so per MMA there are two additions: 32 bytes per
-          // 16-deep step of a K-major operand, 16 rows of 128 bytes of an MN-major one
-          const uint32_t s0 = smem_base + stage * C::STAGE_BYTES;
-          const bool a_mn = ns_is_mn(g_amn, g_asym, row_a, kb), b_mn = ns_is_mn(g_bmn, g_bsym, row_b, kb);
-          const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
-          uint64_t ad = (a_mn ? desc_mn : desc_k) | (s0 >> 4);
-          uint64_t bd = (b_mn ? desc_mn : desc_k) | ((s0 + C::OP_BYTES) >> 4);
-          const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
-#pragma unroll
-          for (int kk = 0; kk < C::BK / 16; ++kk) {
-            if constexpr (CG == 2) umma_ss_pair(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-            else umma_ss(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-            ad += step_a;
-            bd += step_b;
-          }
-          if constexpr (CG == 2) umma_commit_both(&empty_bar[stage]);
-          else umma_commit(&empty_bar[stage]);
+          const int cur = stage;
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1;
           }
+          // 32 bytes per 16-deep step of a K-major operand, 16 rows of 128 bytes of an MN-major one
+          const uint32_t s0 = smem_base + cur * C::STAGE_BYTES;
+          const bool a_mn = ns_is_mn(g_amn, g_asym, row_a, kb), b_mn = ns_is_mn(g_bmn, g_bsym, row_b, kb);
+          const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
+          const uint64_t ad = (a_mn ? desc_mn : desc_k) | (s0 >> 4);
+          const uint64_t bd = (b_mn ? desc_mn : desc_k) | ((s0 + (one ? 0 : C::OP_BYTES)) >> 4);
+          const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < C::BK / 16; ++kk) {
+              if constexpr (CG == 2)
+                umma_ss_pair(d_tmem, ad + kk * step_a, bd + kk * step_b, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+              else umma_ss(d_tmem, ad + kk * step_a, bd + kk * step_b, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            }
+            if constexpr (CG == 2) umma_commit_both(&empty_bar[cur]);
+            else umma_commit(&empty_bar[cur]);
+          }
+          __syncwarp();
         }
         if (!ok) break;
-        if constexpr (CG == 2) umma_commit_both(&accf_bar[acc]);
-        else umma_commit(&accf_bar[acc]);
+        if (leader) {
+          if constexpr (CG == 2) umma_commit_both(&accf_bar[acc]);
+          else umma_commit(&accf_bar[acc]);
+        }
+        __syncwarp();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
-      // All MMAs issued by this thread must finish before TMEM is released.
-      if constexpr (CG == 2) umma_commit_pair_local(&drain_bar);
-      else umma_commit(&drain_bar);
-      mbar_wait(&drain_bar, 0, args.status, 145, nullptr);
+      // All MMAs issued by this warp must finish before TMEM is released.
+      if (leader) {
+        if constexpr (CG == 2) umma_commit_pair_local(&drain_bar);
+        else umma_commit(&drain_bar);
+        mbar_wait(&drain_bar, 0, args.status, 145, nullptr);
+      }
+      __syncwarp();
     }
   } else {
     const int q = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 q.., columns T / 2 half..
