@@ -22,7 +22,7 @@ std::vector<at::Tensor> rmsnorm_fwd(at::Tensor x, at::Tensor w, double eps, bool
 at::Tensor rmsnorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor rstd, c10::optional<at::Tensor> dres,
                        c10::optional<at::Tensor> dx_bf16, at::Tensor dw_out, bool accumulate_dw);
 std::vector<at::Tensor> add_layernorm_fwd(at::Tensor x, c10::optional<at::Tensor> delta, at::Tensor w,
-                                          c10::optional<at::Tensor> b, double eps, bool out_bf16);
+                                          c10::optional<at::Tensor> b, double eps, bool out_bf16, bool stats);
 at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor mean, at::Tensor rstd,
                          c10::optional<at::Tensor> dres, c10::optional<at::Tensor> dx_bf16, at::Tensor dw_out,
                          c10::optional<at::Tensor> db_out, bool accumulate);
@@ -78,7 +78,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("add_rmsnorm_fwd", &pb::add_rmsnorm_fwd);
   m.def("swiglu_bwd_packed", &pb::swiglu_bwd_packed);
   m.def("rmsnorm_bwd", &pb::rmsnorm_bwd);
-  m.def("add_layernorm_fwd", &pb::add_layernorm_fwd);
+  m.def("add_layernorm_fwd", &pb::add_layernorm_fwd, pybind11::arg("x"), pybind11::arg("delta"), pybind11::arg("w"),
+        pybind11::arg("b"), pybind11::arg("eps"), pybind11::arg("out_bf16"), pybind11::arg("stats") = true);
   m.def("layernorm_bwd", &pb::layernorm_bwd);
   m.def("swiglu_fwd", &pb::swiglu_fwd);
   m.def("swiglu_bwd", &pb::swiglu_bwd);

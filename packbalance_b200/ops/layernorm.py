@@ -19,11 +19,17 @@ _TYPES = (torch.float32, torch.bfloat16)
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` as contiguous rows of its last dimension."""
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     return x.reshape(-1, x.shape[-1]).contiguous()
 
 
 def _param(w: torch.Tensor | None) -> torch.Tensor | None:
-    return None if w is None else w.float().contiguous()
+    return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.float().contiguous()
+
+
+def _wants_grad(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, name: str) -> None:
@@ -88,6 +94,9 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     _check(x, weight, bias, "layernorm")
     if not x.is_cuda:
         return layernorm_reference(x, weight, bias, eps)
+    if not _wants_grad(x, weight, bias):  # no autograd node, no saved statistics
+        y = _native.module().add_layernorm_fwd(_rows(x), None, _param(weight), _param(bias), eps, False, False)[1]
+        return y.view(x.shape)
     return _LayerNorm.apply(x, weight, bias, float(eps))
 
 
@@ -104,4 +113,8 @@ def add_layernorm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, bi
     if not x.is_cuda:
         total = x + delta.float()
         return total, layernorm_reference(total, weight, bias, eps).to(torch.bfloat16)
+    if not _wants_grad(x, delta, weight, bias):
+        total, y, _, _ = _native.module().add_layernorm_fwd(_rows(x), _rows(delta), _param(weight), _param(bias), eps,
+                                                            True, False)
+        return total.view(x.shape), y.view(x.shape)
     return _AddLayerNorm.apply(x, delta, weight, bias, float(eps))
