@@ -26,6 +26,9 @@ std::vector<at::Tensor> add_layernorm_fwd(at::Tensor x, c10::optional<at::Tensor
 at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor mean, at::Tensor rstd,
                          c10::optional<at::Tensor> dres, c10::optional<at::Tensor> dx_bf16, at::Tensor dw_out,
                          c10::optional<at::Tensor> db_out, bool accumulate);
+at::Tensor layernorm(at::Tensor x, at::Tensor w, c10::optional<at::Tensor> b, double eps);
+std::vector<at::Tensor> add_layernorm(at::Tensor x, at::Tensor delta, at::Tensor w, c10::optional<at::Tensor> b,
+                                      double eps);
 at::Tensor swiglu_fwd(at::Tensor g, at::Tensor u);
 std::vector<at::Tensor> swiglu_bwd(at::Tensor g, at::Tensor u, at::Tensor dh);
 void rope_apply(at::Tensor x, at::Tensor pos, at::Tensor cos_t, at::Tensor sin_t, int64_t n_rope_cols,
@@ -81,6 +84,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("add_layernorm_fwd", &pb::add_layernorm_fwd, pybind11::arg("x"), pybind11::arg("delta"), pybind11::arg("w"),
         pybind11::arg("b"), pybind11::arg("eps"), pybind11::arg("out_bf16"), pybind11::arg("stats") = true);
   m.def("layernorm_bwd", &pb::layernorm_bwd);
+  m.def("layernorm", &pb::layernorm);
+  m.def("add_layernorm", &pb::add_layernorm);
   m.def("swiglu_fwd", &pb::swiglu_fwd);
   m.def("swiglu_bwd", &pb::swiglu_bwd);
   m.def("rope_apply", &pb::rope_apply);

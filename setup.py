@@ -15,7 +15,7 @@ os.environ.setdefault("MAX_JOBS", str(os.cpu_count() or 4))
 
 ROOT = Path(__file__).parent
 CSRC = ROOT / "packbalance_b200" / "csrc"
-SOURCES = ["bindings.cpp", "gemm.cu", "elementwise.cu", "layernorm.cu", "muon.cu", "attention.cu", "comm.cu", "fsdp.cu", "noalloc.cu"]
+SOURCES = ["bindings.cpp", "gemm.cu", "elementwise.cu", "layernorm.cu", "layernorm_autograd.cpp", "muon.cu", "attention.cu", "comm.cu", "fsdp.cu", "noalloc.cu"]
 SOURCES = [str((CSRC / s).relative_to(ROOT)) for s in SOURCES]
 # PB_DEBUG_BOUNDS=1 builds the index checks of csrc/common.cuh (PB_BOUNDS_OK) into the
 # kernels: a bad work item, owner rank or token id is reported through the device status
