@@ -24,6 +24,8 @@ ATTENTION_BACKENDS = ("auto", "flex", "eager", "sm100")
 PACKING_MODES = ("pad", "pack_random", "pack_ffd", "isoflop")
 SCHEDULES = ("balanced", "random")
 TOKEN_DISTRIBUTIONS = ("uniform", "zipf")
+NORM_TYPES = ("rmsnorm", "layernorm")
+OPTIMIZERS = ("adamw", "muon")
 COMM_BACKENDS = ("auto", "fused", "nccl")
 DTYPES = ("bf16", "fp16", "fp32")
 
@@ -50,8 +52,14 @@ class ModelConfig:
     z_loss_coeff: float = 0.0
     gradient_checkpointing: bool = False
     init_std: float = 0.02
+    # --- additions ---
+    # Normalisation of the decoder: "rmsnorm" (the reference's) or "layernorm" (mean and
+    # variance, weight and bias; replicated parameters, not available with sharding).
+    norm_type: str = "rmsnorm"
 
     def __post_init__(self) -> None:
+        if self.norm_type not in NORM_TYPES:
+            raise ValueError(f"norm_type must be one of {NORM_TYPES}")
         if self.attention_backend not in ATTENTION_BACKENDS:
             raise ValueError(f"attention_backend must be one of {ATTENTION_BACKENDS}")
         if self.d_model % self.n_heads != 0:
@@ -194,8 +202,23 @@ class TrainConfig:
     # -1 (auto) keeps them when they take at most a quarter of the device's memory, else
     # uses two windows.
     fsdp_weight_windows: int = -1
+    # "adamw", or "muon": the decoder layers' weight matrices take orthogonalised momentum
+    # updates (scaled to the size of AdamW's, so lr and weight_decay keep their meaning), every
+    # other parameter AdamW.  Needs whole matrices on every rank, so not with sharding.
+    optimizer: str = "adamw"
+    muon_momentum: float = 0.95
+    muon_nesterov: bool = True
+    muon_steps: int = 5  # Newton-Schulz steps
 
     def __post_init__(self) -> None:
+        if self.optimizer not in OPTIMIZERS:
+            raise ValueError(f"optimizer must be one of {OPTIMIZERS}")
+        if self.optimizer == "muon" and self.fsdp:
+            raise ValueError("optimizer muon needs whole matrices on every rank: not with fsdp")
+        if not 0.0 <= self.muon_momentum < 1.0:
+            raise ValueError("muon_momentum must be in [0, 1)")
+        if not 1 <= self.muon_steps <= 100:
+            raise ValueError("muon_steps must be 1 to 100")
         if self.dtype not in DTYPES:
             raise ValueError("dtype must be bf16, fp16, or fp32")
         if self.max_steps <= 0:

@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(ln_threads(T))
       const int c = (k * T + t) * V;
       if (c < n) {
         put<V>(dx + row * n + c, o + k * V);
-        if constexpr (RES) {
+        if constexpr (sizeof(TI) == 4) {
           if (dx_bf16 != nullptr) put<V>(dx_bf16 + row * n + c, o + k * V);
         }
       }
@@ -880,7 +880,7 @@ at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor m
           if (dr != nullptr)
             done = wide ? launch(std::integral_constant<int, V>{}, std::true_type{})
                         : launch(std::integral_constant<int, 1>{}, std::true_type{});
-          else if (dxb == nullptr)
+          else
             done = wide ? launch(std::integral_constant<int, V>{}, std::false_type{})
                         : launch(std::integral_constant<int, 1>{}, std::false_type{});
         } else if constexpr (!DF) {

@@ -18,6 +18,9 @@ Autograd nodes per step instead of a graph of small ops:
                 that its gradients are final.
 * ``_Head``     final add+RMSNorm + fused LM-head cross-entropy (summed loss).
 
+With ``norm_type: layernorm`` the RMSNorm kernels are replaced by the layer-normalisation
+ones (same fusions; a bias and its gradient, mean and deviation saved per row).
+
 The gradient of ``x + delta`` reaches a layer twice, as the fp32 gradient of ``x``
 and as the bf16 gradient of ``delta``: the bf16 copy is produced by the RMSNorm
 backward kernel and feeds the bf16 GEMMs directly.
@@ -112,9 +115,33 @@ class _Embed(torch.autograd.Function):
         return None, None, None
 
 
+def _add_norm(x, delta, w, b, eps: float, stats: bool = True):
+    """``(x + delta, normalised bf16 rows, row statistics)``: layer normalisation where there
+    is a bias ``b``, else RMSNorm."""
+    C = _native.module()
+    if b is None:
+        x, xn, rstd = C.add_rmsnorm_fwd(x, delta, w, eps, True)
+        return x, xn, (rstd,)
+    x, xn, mean, rstd = C.add_layernorm_fwd(x, delta, w, b, eps, True, stats)
+    return x, xn, (mean, rstd)
+
+
+def _norm_backward(flat: FlatParameters, dxn, x, w, b, stats, dres, dx_bf16):
+    """Gradient of :func:`_add_norm`'s sum (plus ``dres``), fp32 with a bf16 copy; the weight's
+    and bias's gradients go into the flat buffer."""
+    C = _native.module()
+    acc = flat.claim(w)
+    dw = flat.grad_of(w).view(-1)
+    if b is None:
+        return C.rmsnorm_bwd(dxn, x, w, *stats, dres, dx_bf16, dw, acc)
+    if flat.claim(b) != acc:
+        raise RuntimeError("a norm's weight and bias gradients are written together")
+    return C.layernorm_bwd(dxn, x, w, *stats, dres, dx_bf16, dw, flat.grad_of(b).view(-1), acc)
+
+
 def _layer_forward(x_prev, delta_prev, params, sc: StepContext):
     """One decoder layer forward; returns (x1, mlp_out, saved activations)."""
-    w_in, wq, wk, wv, wo, w_post, wg, wu, wd = params
+    w_in, wq, wk, wv, wo, w_post, wg, wu, wd, b_in, b_post = params
     cfg = sc.cfg
     flat = sc.flat
     C = _native.module()
@@ -122,7 +149,7 @@ def _layer_forward(x_prev, delta_prev, params, sc: StepContext):
     h, hk, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
     nqkv = (h + 2 * hk) * hd
     F = cfg.d_ff
-    x, xn1, rstd1 = C.add_rmsnorm_fwd(x_prev, delta_prev, w_in, cfg.norm_eps, True)
+    x, xn1, stats1 = _add_norm(x_prev, delta_prev, w_in, b_in, cfg.norm_eps)
     qkv = torch.empty(t, nqkv, device=x.device, dtype=torch.bfloat16)
     ag = flat.gather_spec(wq, wk, wv)  # sharded weights: fetched inside this GEMM
     gemm(xn1, flat.shadow_of(wq, wk, wv), qkv, t, nqkv, d, epi=EPI_ROPE, pos=sc.pos, cos=sc.cos, sin=sc.sin,
@@ -130,20 +157,21 @@ def _layer_forward(x_prev, delta_prev, params, sc: StepContext):
     o, lse = attn_forward_packed(qkv, sc.plan, h, hk, hd)
     attn_out = torch.empty(t, d, device=x.device, dtype=torch.bfloat16)
     gemm(o, flat.shadow_of(wo), attn_out, t, d, h * hd, epi=EPI_BF16)
-    x1, xn2, rstd2 = C.add_rmsnorm_fwd(x, attn_out, w_post, cfg.norm_eps, True)
+    x1, xn2, stats2 = _add_norm(x, attn_out, w_post, b_post, cfg.norm_eps)
     hmid = torch.empty(t, F, device=x.device, dtype=torch.bfloat16)
     gu = torch.empty(t, 2 * F, device=x.device, dtype=torch.bfloat16)
     ag = flat.gather_spec(wg, wu)
     gemm(xn2, flat.shadow_of(wg, wu), hmid, t, 2 * F, d, epi=EPI_SWIGLU, aux=gu, ag=ag)
     mlp_out = torch.empty(t, d, device=x.device, dtype=torch.bfloat16)
     gemm(hmid, flat.shadow_of(wd), mlp_out, t, d, F, epi=EPI_BF16)
-    return x1, mlp_out, (x, xn1, rstd1, qkv, o, lse, x1, xn2, rstd2, gu, hmid)
+    return x1, mlp_out, (x, xn1, stats1, qkv, o, lse, x1, xn2, stats2, gu, hmid)
 
 
 class _Decoder(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x_prev, delta_prev, w_in, wq, wk, wv, wo, w_post, wg, wu, wd, sc: StepContext):
-        params = (w_in, wq, wk, wv, wo, w_post, wg, wu, wd)
+    def forward(ctx, x_prev, delta_prev, w_in, wq, wk, wv, wo, w_post, wg, wu, wd, b_in, b_post,
+                sc: StepContext):
+        params = (w_in, wq, wk, wv, wo, w_post, wg, wu, wd, b_in, b_post)
         x1, mlp_out, saved = _layer_forward(x_prev, delta_prev, params, sc)
         ctx.sc = sc
         ctx.has_delta = delta_prev is not None
@@ -161,13 +189,12 @@ class _Decoder(torch.autograd.Function):
         sc = ctx.sc
         cfg = sc.cfg
         flat = sc.flat
-        C = _native.module()
-        w_in, wq, wk, wv, wo, w_post, wg, wu, wd = ctx.params
+        w_in, wq, wk, wv, wo, w_post, wg, wu, wd, b_in, b_post = ctx.params
         flat.backward_begin(wq, wk, wv, wo, wg, wu, wd)
         if ctx.saved is None:  # checkpointed: recompute this layer's activations
             ctx.saved = _layer_forward(*ctx.inputs, ctx.params, sc)[2]
             ctx.inputs = None
-        x, xn1, rstd1, qkv, o, lse, x1, xn2, rstd2, gu, hmid = ctx.saved
+        x, xn1, stats1, qkv, o, lse, x1, xn2, stats2, gu, hmid = ctx.saved
         ctx.saved = None
         t, d = x.shape
         h, hk, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
@@ -178,7 +205,7 @@ class _Decoder(torch.autograd.Function):
         dx2b = dx2b.contiguous() if dx2b is not None else dx2.to(torch.bfloat16)
         # one zero fill for the layer's weight gradients (adjacent in the flat buffer), then
         # every weight-gradient writer of the layer accumulates
-        flat.prezero(wq, wk, wv, wo, w_post, wg, wu, wd)
+        flat.prezero(wq, wk, wv, wo, w_post, *(() if b_post is None else (b_post,)), wg, wu, wd)
         # MLP
         # down-projection dgrad with the SwiGLU backward in its epilogue: [dg | du]
         dgu = torch.empty(t, 2 * F, device=dev, dtype=torch.bfloat16)
@@ -188,7 +215,7 @@ class _Decoder(torch.autograd.Function):
         gemm(dgu, flat.shadow_of(wg, wu), dxn2, t, d, 2 * F, b_mn=True, epi=EPI_F32)
         _wgrad(flat, (wg, wu), dgu, xn2)
         dx1b = torch.empty(t, d, device=dev, dtype=torch.bfloat16)
-        dx1 = C.rmsnorm_bwd(dxn2, x1, w_post, rstd2, dx2, dx1b, flat.grad_of(w_post).view(-1), flat.claim(w_post))
+        dx1 = _norm_backward(flat, dxn2, x1, w_post, b_post, stats2, dx2, dx1b)
         # attention
         do = torch.empty(t, h * hd, device=dev, dtype=torch.bfloat16)
         gemm(dx1b, flat.shadow_of(wo), do, t, h * hd, d, b_mn=True, epi=EPI_BF16)
@@ -198,10 +225,10 @@ class _Decoder(torch.autograd.Function):
         gemm(dqkv, flat.shadow_of(wq, wk, wv), dxn1, t, d, nqkv, b_mn=True, epi=EPI_F32)
         _wgrad(flat, (wq, wk, wv), dqkv, xn1)
         dxb = torch.empty(t, d, device=dev, dtype=torch.bfloat16)
-        dx = C.rmsnorm_bwd(dxn1, x, w_in, rstd1, dx1, dxb, flat.grad_of(w_in).view(-1), flat.claim(w_in))
+        dx = _norm_backward(flat, dxn1, x, w_in, b_in, stats1, dx1, dxb)
         _join_wgrads(dev)
         flat.ready_after(w_in)
-        return (dx, dxb if ctx.has_delta else None) + (None,) * 10
+        return (dx, dxb if ctx.has_delta else None) + (None,) * 12
 
 
 # The LM head can keep its bf16 logits for the backward (one elementwise pass instead
@@ -214,10 +241,9 @@ LOGITS_KEEP_BYTES = 0
 
 class _Head(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x_prev, delta_prev, w_norm, w_lm, labels, sc: StepContext):
+    def forward(ctx, x_prev, delta_prev, w_norm, b_norm, w_lm, labels, sc: StepContext):
         cfg = sc.cfg
-        C = _native.module()
-        x, xf, rstd = C.add_rmsnorm_fwd(x_prev, delta_prev, w_norm, cfg.norm_eps, True)
+        x, xf, stats = _add_norm(x_prev, delta_prev, w_norm, b_norm, cfg.norm_eps)
         ag = sc.flat.gather_spec(w_lm)
         t = xf.shape[0]
         keep = t * cfg.vocab_size * 2 <= LOGITS_KEEP_BYTES and cfg.vocab_size % 8 == 0
@@ -227,8 +253,8 @@ class _Head(torch.autograd.Function):
         ctx.sc = sc
         ctx.has_delta = delta_prev is not None
         ctx.logits = logits
-        ctx.saved = (x, xf, rstd, lse, labels)
-        ctx.params = (w_norm, w_lm)
+        ctx.saved = (x, xf, stats, lse, labels)
+        ctx.params = (w_norm, b_norm, w_lm)
         return loss
 
     @staticmethod
@@ -236,19 +262,23 @@ class _Head(torch.autograd.Function):
         sc = ctx.sc
         cfg = sc.cfg
         flat = sc.flat
-        x, xf, rstd, lse, labels = ctx.saved
+        x, xf, stats, lse, labels = ctx.saved
         ctx.saved = None
-        w_norm, w_lm = ctx.params
+        w_norm, b_norm, w_lm = ctx.params
         dxf = lmhead_ce_backward(
             xf, flat.shadow_of(w_lm), labels, lse, grad, flat.grad_of(w_lm), flat.claim(w_lm), -100, cfg.z_loss_coeff,
             logits=ctx.logits,
         )
         ctx.logits = None
         dxb = torch.empty(x.shape, device=x.device, dtype=torch.bfloat16)
-        dx = _native.module().rmsnorm_bwd(dxf, x, w_norm, rstd, None, dxb, flat.grad_of(w_norm).view(-1),
-                                          flat.claim(w_norm))
+        dx = _norm_backward(flat, dxf, x, w_norm, b_norm, stats, None, dxb)
         flat.ready_after(w_norm)
-        return dx, (dxb if ctx.has_delta else None), None, None, None, None
+        return dx, (dxb if ctx.has_delta else None), None, None, None, None, None
+
+
+def _bias(norm) -> torch.Tensor | None:
+    """The bias of a layer normalisation; None for RMSNorm."""
+    return getattr(norm, "bias", None)
 
 
 def _ensure_flat(model):
@@ -279,13 +309,13 @@ def fused_causal_lm_forward(model, input_ids, labels, position_ids, doc_start, a
         x, delta = _Decoder.apply(
             x, delta, layer.input_layernorm.weight, a.q_proj.weight, a.k_proj.weight, a.v_proj.weight,
             a.o_proj.weight, layer.post_attention_layernorm.weight, mlp.gate_proj.weight, mlp.up_proj.weight,
-            mlp.down_proj.weight, sc,
+            mlp.down_proj.weight, _bias(layer.input_layernorm), _bias(layer.post_attention_layernorm), sc,
         )
     shape = input_ids.shape
     if labels is not None:
-        loss = _Head.apply(x, delta, m.norm.weight, model.lm_head_weight, labels.reshape(-1).contiguous(), sc)
+        loss = _Head.apply(x, delta, m.norm.weight, _bias(m.norm), model.lm_head_weight, labels.reshape(-1).contiguous(), sc)
         return CausalLMOutput(loss=loss, hidden_states=None)
-    _, xf, _ = _native.module().add_rmsnorm_fwd(x, delta, m.norm.weight, cfg.norm_eps, True)
+    _, xf, _ = _add_norm(x, delta, m.norm.weight, _bias(m.norm), cfg.norm_eps, stats=False)
     w = flat.shadow_of(model.lm_head_weight)
     logits = torch.empty(xf.shape[0], cfg.vocab_size, device=xf.device, dtype=torch.bfloat16)
     gemm(xf, w, logits, xf.shape[0], cfg.vocab_size, cfg.d_model, epi=EPI_BF16)

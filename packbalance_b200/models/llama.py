@@ -1,7 +1,7 @@
 """Llama-style decoder for packed-sequence training.
 
 Architecture and parameter names follow the reference (``model/llama.py:36-290``):
-pre-norm RMSNorm, GQA attention with RoPE on per-document positions, SwiGLU MLP,
+pre-norm RMSNorm (or, by ``norm_type``, layer normalisation), GQA attention with RoPE on per-document positions, SwiGLU MLP,
 tied embeddings by default, N(0, init_std) init with residual projections scaled by
 1/sqrt(2 * n_layers).  ``forward`` returns the *summed* token cross-entropy (plus
 z-loss) when labels are given, otherwise logits.
@@ -31,6 +31,7 @@ from packbalance_b200.models.attention import attention_forward, doc_start_from_
 from packbalance_b200.models.rope import RotaryEmbedding
 from packbalance_b200.ops.reference import (
     chunked_linear_cross_entropy,
+    layernorm_reference,
     rmsnorm_reference,
     rope_reference,
     swiglu_reference,
@@ -57,6 +58,28 @@ class RMSNorm(nn.Module):
 
             return rmsnorm(x, self.weight, self.eps)
         return rmsnorm_reference(x, self.weight, self.eps)
+
+
+class LayerNorm(nn.Module):
+    def __init__(self, d_model: int, eps: float, use_fused: bool = True) -> None:
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(d_model))
+        self.bias = nn.Parameter(torch.zeros(d_model))
+        self.eps = eps
+        self.use_fused = use_fused
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.is_cuda and self.use_fused:
+            from packbalance_b200.ops.layernorm import layernorm
+
+            return layernorm(x, self.weight, self.bias, self.eps)
+        return layernorm_reference(x, self.weight, self.bias, self.eps)
+
+
+def make_norm(cfg: ModelConfig) -> nn.Module:
+    """The normalisation ``cfg.norm_type`` names, over ``d_model``."""
+    kind = LayerNorm if cfg.norm_type == "layernorm" else RMSNorm
+    return kind(cfg.d_model, cfg.norm_eps, cfg.use_fused_rmsnorm)
 
 
 class LlamaMLP(nn.Module):
@@ -156,9 +179,9 @@ class LlamaDecoderLayer(nn.Module):
 
     def __init__(self, cfg: ModelConfig) -> None:
         super().__init__()
-        self.input_layernorm = RMSNorm(cfg.d_model, cfg.norm_eps, cfg.use_fused_rmsnorm)
+        self.input_layernorm = make_norm(cfg)
         self.self_attn = LlamaAttention(cfg)
-        self.post_attention_layernorm = RMSNorm(cfg.d_model, cfg.norm_eps, cfg.use_fused_rmsnorm)
+        self.post_attention_layernorm = make_norm(cfg)
         self.mlp = LlamaMLP(cfg)
 
     def forward(self, hidden, cos, sin, doc_ids, block_mask=None, cache: tuple[KVCache, int] | None = None):
@@ -173,7 +196,7 @@ class LlamaModel(nn.Module):
         self.cfg = cfg
         self.embed_tokens = nn.Embedding(cfg.vocab_size, cfg.d_model)
         self.layers = nn.ModuleList(LlamaDecoderLayer(cfg) for _ in range(cfg.n_layers))
-        self.norm = RMSNorm(cfg.d_model, cfg.norm_eps, cfg.use_fused_rmsnorm)
+        self.norm = make_norm(cfg)
         self.rotary = RotaryEmbedding(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta)
         self.gradient_checkpointing = False
 

@@ -11,7 +11,7 @@ scalars (no host synchronisation):
    global-token normalisation, ``train/train.py:320-345``);
 3. backward writes weight gradients into the flat buffer; the data-parallel engine
    averages them bucket by bucket as layers finish;
-4. global gradient norm, clipping and AdamW run as device kernels; a non-finite
+4. global gradient norm, clipping and AdamW (or Muon) run as device kernels; a non-finite
    norm skips the update.
 
 On the native CUDA path without sharding, the whole step (forward, backward, the
@@ -39,7 +39,7 @@ from packbalance_b200.models.llama import LlamaForCausalLM
 from packbalance_b200.ops.attention import PLAN_CTAS, attention_plan_host, plan_to_device
 from packbalance_b200.parallel.distributed import DataParallel
 from packbalance_b200.parallel.flat import FlatParameters
-from packbalance_b200.parallel.optim import FlatAdamW, global_grad_norm
+from packbalance_b200.parallel.optim import FlatAdamW, FlatMuon, global_grad_norm, hidden_matrices
 from packbalance_b200.utils import get_autocast_dtype, get_world_size
 
 
@@ -206,6 +206,10 @@ class TrainEngine:
             self.model.gradient_checkpointing_enable()
         self.model.train()
         self.fsdp = bool(cfg.train.fsdp) and self.world > 1
+        if cfg.train.fsdp and cfg.train.optimizer == "muon":
+            raise ValueError("train.optimizer muon needs whole matrices on every rank: not with train.fsdp")
+        if self.fsdp and device.type == "cuda" and cfg.model.norm_type == "layernorm":
+            raise ValueError("model.norm_type layernorm is not available with train.fsdp on CUDA")
         self.sharded = None
         native_ok = device.type == "cuda" and self.model.uses_native_path(torch.empty(0, device=device))
         # the reference's train.deterministic: fixed-order reductions in the native kernels
@@ -262,12 +266,13 @@ class TrainEngine:
             self.dp = DataParallel(self.flat, cfg.train.bucket_cap_mb, cfg.train.comm_backend,
                                    deterministic=self.deterministic, wire=cfg.train.grad_reduce_dtype)
             self.flat.ready_hook = self.dp.notify_ready
-            self.optimizer = FlatAdamW(
-                self.flat,
-                lr=cfg.train.lr,
-                betas=(cfg.train.beta1, cfg.train.beta2),
-                weight_decay=cfg.train.weight_decay,
-            )
+            hyper = dict(lr=cfg.train.lr, betas=(cfg.train.beta1, cfg.train.beta2),
+                         weight_decay=cfg.train.weight_decay)
+            if cfg.train.optimizer == "muon":
+                self.optimizer = FlatMuon(self.flat, hidden_matrices(self.model), momentum=cfg.train.muon_momentum,
+                                          nesterov=cfg.train.muon_nesterov, muon_steps=cfg.train.muon_steps, **hyper)
+            else:
+                self.optimizer = FlatAdamW(self.flat, **hyper)
         self.scheduler = self.make_scheduler(start_step)
         self.native = self.model.uses_native_path(torch.empty(0, device=device))
         self._graphs: dict[tuple, _GraphedStep] = {}
