@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ Pa
   __shared__ double red[8];
   int local;
   const PassGroup& g = a.g[pass_group(a, blockIdx.x, local)];
+  grid_dependency_wait();
   float s;
   if (!clip_factor(a, s)) return;
   const int mat = local / g.chunks;
@@ -425,17 +426,19 @@ void ns_launch(const NsArgs& args, const Step& step, int dev, cudaStream_t strea
   using C = NsCfg<CG>;
   auto kern = ns_gemm_kernel<CG, MODE, Step>;
   static int max_clusters[64] = {0};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see grid_dependency_wait
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(C::THREADS, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
+  cfg.numAttrs = CG == 2 ? 2 : 1;
   if (max_clusters[dev] == 0) {
     PB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
     int n = num_sms(dev) / CG;
@@ -606,8 +609,16 @@ template <typename TG, bool MOM>
 void ns_passes(PassArgs& a, const MatTable& t, int blocks, cudaStream_t s) {
   ns_norm_kernel<TG, MOM><<<blocks, 256, 0, s>>>(a, t);
   PB_CUDA_CHECK(cudaGetLastError());
-  ns_init_kernel<TG, MOM><<<blocks, 256, 0, s>>>(a, t);
-  PB_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_init_kernel<TG, MOM>, a, t));
 }
 
 int64_t chunks_of(const Shape& s) { return (s.rows * s.cols + kChunk - 1) / kChunk; }

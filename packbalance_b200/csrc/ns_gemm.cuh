@@ -111,6 +111,9 @@ __device__ __forceinline__ uint32_t ns_idesc(int t, int a_mn, int b_mn) {
          (static_cast<uint32_t>(t >> 3) << 17) | (static_cast<uint32_t>(t >> 4) << 24);
 }
 
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependents_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 struct NsTile {
   int g, mat, i, j;
 };
@@ -249,11 +252,39 @@ __device__ __forceinline__ float ns_block_at(const float* s, int r, int c) {
   return s[r * 32 + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3))];
 }
 
-// Epilogue of one tile for the 32 rows from ``row0`` and the tile columns [c0, c0 + T / 2);
-// ``tacc`` is the accumulator's address at those rows and columns.
+// What the epilogue of ``tile`` will read for this warp's rows (the low part, the parameters)
+// starts moving into L2 while the tile before it is finished: both are larger than L2 and the
+// DRAM latency was otherwise paid once per 32 columns.
 template <int CG, int MODE, class Step>
-__device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, const NsTile& t, typename NsCfg<CG>::Stg& st,
-                                            uint32_t tacc, int row0, int c0) {
+__device__ __forceinline__ void ns_prefetch(const NsArgs& a, const Step& sa, int tile, int row_in_tile, int c0) {
+  using C = NsCfg<CG>;
+  if constexpr (MODE == NS_APPLY || MODE == NS_STEP) {
+    if (tile >= a.tiles) return;
+    const NsTile t = ns_tile<CG, false>(a, tile);
+    const NsGroup& g = a.g[t.g];
+    const int row = t.i * C::T + row_in_tile, col = t.j * C::T + c0;
+    if (row >= g.M) return;
+    const char* p = nullptr;
+    int piece = 0;  // columns per 128-byte line
+    if constexpr (MODE == NS_APPLY) {
+      if (g.add == nullptr) return;
+      p = reinterpret_cast<const char*>(g.add + t.mat * g.add_batch + static_cast<long>(row) * g.add_ld + col);
+      piece = 64;
+    } else {
+      p = reinterpret_cast<const char*>(sa.p[g.mat0 + t.mat] + static_cast<long>(row) * g.N + col);
+      piece = 32;
+    }
+    for (int c = 0; c < C::T / 2 && col + c < g.N; c += piece, p += 128)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+  }
+}
+
+// Epilogue of one tile for the 32 rows from ``row0`` and the tile columns [c0, c0 + T / 2);
+// ``tacc`` is the accumulator's address at those rows and columns.  Inputs that do not depend on
+// the products are requested before ``wait()`` waits for the accumulator (false: give up).
+template <int CG, int MODE, class Step, class Wait>
+__device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, const NsTile& t, typename NsCfg<CG>::Stg& st,
+                                            uint32_t tacc, int row0, int c0, Wait&& wait) {
   using C = NsCfg<CG>;
   constexpr int W = C::T / 2;
   const NsGroup& g = a.g[t.g];
@@ -263,21 +294,29 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
   if constexpr (MODE == NS_GRAM || MODE == NS_POLY || MODE == NS_APPLY) {
     const bool with_add = MODE != NS_GRAM && g.add != nullptr;
     const bool ok = with_add && row < g.M;
-    const __half* arow = with_add ? g.add + t.mat * g.add_batch + static_cast<long>(ok ? row : 0) * g.add_ld : nullptr;
-    uint4 q[4];
-    if (with_add) ns_load_add(arow, ok, col0, g.add_ld, q);
-    tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
-      const int col = col0 + c;
-      if (col >= g.N) return;  // uniform across the warp
+    uint4 q[W / 32][4];
+    if constexpr (MODE != NS_GRAM) {
       if (with_add) {
-        uint4 qn[4];
-        if (c + 32 < W) ns_load_add(arow, ok, col + 32, g.add_ld, qn);
-        ns_add(v, q, a.alpha, a.beta);
-        if (c + 32 < W) {
+        const __half* arow = g.add + t.mat * g.add_batch + static_cast<long>(ok ? row : 0) * g.add_ld;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) q[j] = qn[j];
+        for (int k = 0; k < W / 32; ++k) ns_load_add(arow, ok, col0 + 32 * k, g.add_ld, q[k]);
+      }
+    }
+    if (!wait()) return false;
+#pragma unroll
+    for (int k = 0; k < W / 32; ++k) {
+      const int col = col0 + 32 * k;
+      if (col >= g.N) break;  // uniform across the warp
+      float v[32];
+      tmem_load_f32(tacc + 32 * k, v);
+      bool added = false;
+      if constexpr (MODE != NS_GRAM) {
+        if (with_add) {
+          ns_add(v, q[k], a.alpha, a.beta);
+          added = true;
         }
-      } else {
+      }
+      if (!added) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= a.alpha;
       }
@@ -302,8 +341,9 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
           st.release();
         }
       }
-    });
+    }
   } else if constexpr (MODE == NS_LAST) {
+    if (!wait()) return false;
     if (g.dst_tma) {
       tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
         const int col = col0 + c;
@@ -331,7 +371,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
   } else {
     // The parameters of the next 32 columns are on their way while this block is updated: the
     // launch reads and writes 4 bytes per element, more than its products cost.
-    if (sa.norm != nullptr && !isfinite(*sa.norm)) return;
+    if (sa.norm != nullptr && !isfinite(*sa.norm)) return wait();
     const float lr = sa.hp != nullptr ? *sa.hp : sa.lr;
     const float decay = 1.f - lr * sa.weight_decay;
     const float step = lr * g.step * a.alpha;
@@ -339,9 +379,10 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
     __nv_bfloat16* sh = sa.shadow[g.mat0 + t.mat];
     float* s = reinterpret_cast<float*>(st.base);
     if (g.vec) {
-      // a lane takes the 16-byte piece lane % 8 of rows lane / 8, + 4, + 8, ...
+      // a lane takes the 16-byte piece lane % 8 of rows lane / 8, + 4, + 8, ...; two blocks of
+      // 32 columns are on their way
       const int r0 = lane >> 3, q = lane & 7;
-      float4 cur[8], next[8];
+      float4 buf[2][8];
       auto fetch = [&](int col, float4 (&w)[8]) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -349,12 +390,13 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
                      ? *reinterpret_cast<const float4*>(p + static_cast<long>(row0 + r0 + 4 * k) * g.N + col + 4 * q)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
       };
-      fetch(col0, cur);
-#pragma unroll 1
+      fetch(col0, buf[0]);
+      fetch(col0 + 32, buf[1]);
+      if (!wait()) return false;
+#pragma unroll
       for (int c = 0; c < W; c += 32) {
         const int col = col0 + c;
         if (col >= g.N) break;  // uniform across the warp
-        if (c + 32 < W) fetch(col + 32, next);
         {
           float v[32];
           tmem_load_f32(tacc + c, v);
@@ -364,7 +406,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
         for (int k = 0; k < 8; ++k) {
           const int r = r0 + 4 * k;
           const float4 o = ns_block_piece(s, r, q);
-          float4 w = cur[k];
+          float4 w = buf[c / 32 & 1][k];
           w.x = w.x * decay - step * o.x;
           w.y = w.y * decay - step * o.y;
           w.z = w.z * decay - step * o.z;
@@ -375,11 +417,12 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
             if (sh != nullptr)
               *reinterpret_cast<uint2*>(sh + at) = make_uint2(pack_bf16x2(w.x, w.y), pack_bf16x2(w.z, w.w));
           }
-          cur[k] = next[k];
         }
+        if (c + 64 < W) fetch(col + 64, buf[c / 32 & 1]);
         __syncwarp();
       }
     } else {
+      if (!wait()) return false;
       const int rows = min(32, g.M - row0);
       tmem_walk(tacc, W, [&](int c, float (&v)[32]) {
         const int col = col0 + c;
@@ -406,6 +449,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, const Step& sa, con
       });
     }
   }
+  return true;
 }
 
 // NsCfg::THREADS threads; CG == 2 with cluster dimension (2, 1, 1).
@@ -458,6 +502,10 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
+  // The launch before this one may still be finishing on other SMs: everything above overlaps its
+  // tail, everything below reads what it wrote.
+  grid_dependency_wait();
+  grid_dependents_go();
 
   // Warps 0 and 1 run their loops with all lanes converged and elect one to issue.  A k-block's
   // MMAs take 512 cycles; measured per k-block the issuing warp spends about 190 on its barrier,
@@ -608,16 +656,25 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
     const int q = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 q.., columns T / 2 half..
     const uint32_t acce0 = CG == 2 ? cluster_addr(smem_u32(&acce_bar[0]), 0) : 0;
     typename C::Stg st{smem + C::EPI_OFF + (warp - 2) * C::Stg::kBytes, 0, false};
+    const int row_in_tile = static_cast<int>(cta) * C::BM + q * 32;
     int acc = 0;
     uint32_t acc_phase = 0;
+    ns_prefetch<CG, MODE>(args, step, first, row_in_tile + lane, half * (C::T / 2));
     for (int tile = first; tile < args.tiles; tile += stride) {
       const NsTile t = ns_tile<CG, SYM>(args, tile);
-      if (!mbar_wait_warp(&accf_bar[acc], acc_phase, args.status, 146, &abort_sh)) break;
-      tc_fence_after();
       const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::T + half * (C::T / 2);
-      const int row0 = t.i * C::T + static_cast<int>(cta) * C::BM + q * 32;
+      const int row0 = t.i * C::T + row_in_tile;
+      auto wait = [&] {
+        const bool ok = mbar_wait_warp(&accf_bar[acc], acc_phase, args.status, 146, &abort_sh);
+        tc_fence_after();
+        return ok;
+      };
+      ns_prefetch<CG, MODE>(args, step, tile + stride, row_in_tile + lane, half * (C::T / 2));
+      bool ok;
       if (row0 < args.g[t.g].M && t.j * C::T + half * (C::T / 2) < args.g[t.g].N)
-        ns_epilogue<CG, MODE>(args, step, t, st, tacc, row0, half * (C::T / 2));
+        ok = ns_epilogue<CG, MODE>(args, step, t, st, tacc, row0, half * (C::T / 2), wait);
+      else ok = wait();
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
