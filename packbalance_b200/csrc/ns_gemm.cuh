@@ -379,46 +379,49 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
     __nv_bfloat16* sh = sa.shadow[g.mat0 + t.mat];
     float* s = reinterpret_cast<float*>(st.base);
     if (g.vec) {
-      // a lane takes the 16-byte piece lane % 8 of rows lane / 8, + 4, + 8, ...; two blocks of
-      // 32 columns are on their way
+      // A lane takes the 16-byte piece lane % 8 of rows lane / 8, + 4, + 8, ...; as a piece is
+      // used, the one 32 columns on is requested into its registers.  (Holding two blocks ahead
+      // spilled, and with 225 KB of shared memory in use a spill's reload comes from L2: 253 us
+      // instead of %STEP% for the 100M model's last product.)
       const int r0 = lane >> 3, q = lane & 7;
-      float4 buf[2][8];
-      auto fetch = [&](int col, float4 (&w)[8]) {
+      const int rows = (g.M - row0 - r0 + 3) / 4;  // this lane's rows in range
+      const long base = static_cast<long>(row0 + r0) * g.N + col0 + 4 * q;
+      const int pitch = 4 * g.N, cols = g.N - col0 - 4 * q;
+      const float* next = p + base;
+      float4 buf[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          w[k] = row0 + r0 + 4 * k < g.M && col + 4 * q < g.N
-                     ? *reinterpret_cast<const float4*>(p + static_cast<long>(row0 + r0 + 4 * k) * g.N + col + 4 * q)
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
-      };
-      fetch(col0, buf[0]);
-      fetch(col0 + 32, buf[1]);
+      for (int k = 0; k < 8; ++k) {
+        buf[k] = k < rows && cols > 0 ? *reinterpret_cast<const float4*>(next) : make_float4(0.f, 0.f, 0.f, 0.f);
+        next += pitch;
+      }
       if (!wait()) return false;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < W; c += 32) {
-        const int col = col0 + c;
-        if (col >= g.N) break;  // uniform across the warp
+        if (col0 + c >= g.N) break;  // uniform across the warp
         {
           float v[32];
           tmem_load_f32(tacc + c, v);
           ns_block_in(s, v);
         }
+        float* at = p + base + c;
+        __nv_bfloat16* to = sh + base + c;
+        const bool more = c + 32 < W && cols > c + 32;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int r = r0 + 4 * k;
-          const float4 o = ns_block_piece(s, r, q);
-          float4 w = buf[c / 32 & 1][k];
+          const float4 o = ns_block_piece(s, r0 + 4 * k, q);
+          float4 w = buf[k];
+          if (more && k < rows) buf[k] = *reinterpret_cast<const float4*>(at + 32);
           w.x = w.x * decay - step * o.x;
           w.y = w.y * decay - step * o.y;
           w.z = w.z * decay - step * o.z;
           w.w = w.w * decay - step * o.w;
-          if (row0 + r < g.M && col + 4 * q < g.N) {
-            const long at = static_cast<long>(row0 + r) * g.N + col + 4 * q;
-            *reinterpret_cast<float4*>(p + at) = w;
-            if (sh != nullptr)
-              *reinterpret_cast<uint2*>(sh + at) = make_uint2(pack_bf16x2(w.x, w.y), pack_bf16x2(w.z, w.w));
+          if (k < rows && cols > c) {
+            *reinterpret_cast<float4*>(at) = w;
+            if (sh != nullptr) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(w.x, w.y), pack_bf16x2(w.z, w.w));
           }
+          at += pitch;
+          to += pitch;
         }
-        if (c + 64 < W) fetch(col + 64, buf[c / 32 & 1]);
         __syncwarp();
       }
     } else {
