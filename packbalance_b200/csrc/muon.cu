@@ -523,52 +523,53 @@ void ns_iterate(std::vector<Shape>& shapes, const Iteration& it, int dev, cudaSt
     apply.g[k].mat0 = at;
     at += (int)shapes[k].batch();
   }
+  // everything but which of the two X buffers is read is the same in every step
+  std::vector<std::array<CUtensorMap, 2>> x_load(n), x_store(n);
+  for (int k = 0; k < n; ++k) {
+    Shape& sh = shapes[k];
+    const int64_t r = sh.r(), B = sh.batch();
+    for (int i = 0; i < (it.steps > 1 ? 2 : 1); ++i) {
+      x_load[k][i] = load_map(sh.x[i], sh.cols, sh.rows, B, sh.ld());
+      x_store[k][i] = store_map(sh.x[i], sh.cols, sh.rows, B, sh.ld(), false);
+    }
+    NsGroup& g = gram.g[k];
+    g.a_mn = g.b_mn = sh.tall();
+    g.M = g.N = (int)r;
+    g.K = (int)std::max(sh.rows, sh.cols);
+    g.out = store_map(sh.gram, r, r, B, sh.ldr(), false);
+    NsGroup& q = poly.g[k];
+    q.a = q.b = load_map(sh.gram, r, r, B, sh.ldr());
+    q.out = store_map(sh.poly, r, r, B, sh.ldr(), false);
+    q.add = sh.gram;
+    q.add_batch = r * sh.ldr();
+    q.add_ld = (int)sh.ldr();
+    q.a_sym = q.b_sym = 1;
+    q.M = q.N = q.K = (int)r;
+    NsGroup& y = apply.g[k];
+    (sh.tall() ? y.b : y.a) = load_map(sh.poly, r, r, B, sh.ldr());
+    y.a_sym = !sh.tall();
+    y.b_sym = sh.tall();
+    y.b_mn = !sh.tall();
+    y.M = (int)sh.rows;
+    y.N = (int)sh.cols;
+    y.K = (int)r;
+    y.add_batch = sh.rows * sh.low_ld();
+    y.add_ld = (int)sh.low_ld();
+    if (it.steps > 3)
+      y.low = map3(sh.low, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, sh.cols, sh.rows, B, sh.low_ld(), 32,
+                   CU_TENSOR_MAP_SWIZZLE_NONE);
+    for (NsGroup* p : {&g, &q, &y}) p->k_blocks = (p->K + 63) / 64;
+  }
   for (int step = 0, cur = 0; step < it.steps; ++step, cur ^= 1) {
     const bool final = step + 1 == it.steps;
     for (int k = 0; k < n; ++k) {
-      Shape& sh = shapes[k];
-      const int64_t r = sh.r(), B = sh.batch();
-      const CUtensorMap x = load_map(sh.x[cur], sh.cols, sh.rows, B, sh.ld());
-      NsGroup& g = gram.g[k];
-      g.a = g.b = x;
-      g.a_mn = g.b_mn = sh.tall();
-      g.M = g.N = (int)r;
-      g.K = (int)std::max(sh.rows, sh.cols);
-      g.k_blocks = (g.K + 63) / 64;
-      NsGroup& q = poly.g[k];
-      if (step == 0) {
-        g.out = store_map(sh.gram, r, r, B, sh.ldr(), false);
-        q.a = q.b = load_map(sh.gram, r, r, B, sh.ldr());
-        q.out = store_map(sh.poly, r, r, B, sh.ldr(), false);
-        q.add = sh.gram;
-        q.add_batch = r * sh.ldr();
-        q.add_ld = (int)sh.ldr();
-        q.a_sym = q.b_sym = 1;
-        q.M = q.N = q.K = (int)r;
-        q.k_blocks = (q.K + 63) / 64;
-      }
+      gram.g[k].a = gram.g[k].b = x_load[k][cur];
       NsGroup& y = apply.g[k];
-      const CUtensorMap p = load_map(sh.poly, r, r, B, sh.ldr());
-      y.a = sh.tall() ? x : p;
-      y.b = sh.tall() ? p : x;
-      y.a_sym = !sh.tall();
-      y.b_sym = sh.tall();
-      y.b_mn = !sh.tall();
-      y.M = (int)sh.rows;
-      y.N = (int)sh.cols;
-      y.K = (int)r;
-      y.k_blocks = (y.K + 63) / 64;
+      (shapes[k].tall() ? y.a : y.b) = x_load[k][cur];
       // the input carries a low part while at least two steps follow this one
-      y.low_in = step + 2 < it.steps ? sh.low : nullptr;
-      y.add_batch = sh.rows * sh.low_ld();
-      y.add_ld = (int)sh.low_ld();
+      y.low_in = step + 2 < it.steps ? shapes[k].low : nullptr;
       y.store_low = step + 3 < it.steps;
-      if (!final) {
-        y.out = store_map(sh.x[cur ^ 1], sh.cols, sh.rows, B, sh.ld(), false);
-        if (y.store_low)
-          y.low = map3(sh.low, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, sh.cols, sh.rows, B, sh.low_ld(), 32,
-                       CU_TENSOR_MAP_SWIZZLE_NONE);
-      }
+      if (!final) y.out = x_store[k][cur ^ 1];
     }
     ns_product<NS_GRAM>(gram, NsNoStep{}, dev, s);
     ns_product<NS_POLY>(poly, NsNoStep{}, dev, s);

@@ -174,6 +174,29 @@ __device__ __forceinline__ void ns_load_operand(uint8_t* dst, const CUtensorMap*
   ns_load<CG>(dst + 8192, map, bar, mn ? x + 64 : x, mn ? y : y + 64, mat);
 }
 
+// One MMA; the operands' shared-memory descriptors share their high word (stride 1024, version,
+// swizzle) and are put together here.
+template <int CG>
+__device__ __forceinline__ void ns_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t ok;
@@ -643,7 +666,7 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
       uint32_t acc_phase = 0;
       bool ok = true;
       const uint32_t smem_base = smem_u32(smem);
-      const uint64_t desc_k = sdesc_sw128(0, 16, 1024), desc_mn = sdesc_sw128(0, 8192, 1024);
+      const uint32_t desc_hi = static_cast<uint32_t>(sdesc_sw128(0, 0, 1024) >> 32);
       for (int tile = first; tile < args.tiles && ok; tile += stride) {
         const NsTile t = ns_tile<CG, SYM>(args, tile);
         const NsGroup& g = args.g[t.g];
@@ -653,35 +676,40 @@ __global__ void __launch_bounds__(NsCfg<CG>::THREADS, 1)
         if (!mbar_wait_warp(&acce_bar[acc], acc_phase ^ 1, args.status, 143, &abort_sh)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * C::T;
-        for (int kb = 0; kb < kbs; ++kb) {
-          if (!ns_wait(&full_bar[stage], phase, args.status, 144, &abort_sh)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const int cur = stage;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
-          // 32 bytes per 16-deep step of a K-major operand, 16 rows of 128 bytes of an MN-major one
-          const uint32_t s0 = smem_base + cur * C::STAGE_BYTES;
-          const bool a_mn = ns_is_mn(g_amn, g_asym, row_a, kb), b_mn = ns_is_mn(g_bmn, g_bsym, row_b, kb);
+        // A symmetric operand is MN-major below its diagonal block and K-major from there on, so
+        // the k-blocks fall into at most three runs of one kind each; within a run only the stage
+        // address changes.
+        const int cut_a = g_asym ? min(kbs, row_a / 256 * 4) : (g_amn ? kbs : 0);
+        const int cut_b = g_bsym ? min(kbs, row_b / 256 * 4) : (g_bmn ? kbs : 0);
+        for (int kb = 0; kb < kbs && ok;) {
+          const bool a_mn = kb < cut_a, b_mn = kb < cut_b;
+          const int end = min(a_mn ? cut_a : kbs, b_mn ? cut_b : kbs);
           const uint32_t idesc = ns_idesc(C::T, a_mn, b_mn);
-          const uint64_t ad = (a_mn ? desc_mn : desc_k) | (s0 >> 4);
-          const uint64_t bd = (b_mn ? desc_mn : desc_k) | ((s0 + (one ? 0 : C::OP_BYTES)) >> 4);
-          const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
-          if (leader) {
-#pragma unroll
-            for (int kk = 0; kk < C::BK / 16; ++kk) {
-              if constexpr (CG == 2)
-                umma_ss_pair(d_tmem, ad + kk * step_a, bd + kk * step_b, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-              else umma_ss(d_tmem, ad + kk * step_a, bd + kk * step_b, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          // 32 bytes per 16-deep step of a K-major operand, 16 rows of 128 bytes of an MN-major one
+          const uint32_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+          const uint32_t a_lbo = (a_mn ? 8192u : 16u) >> 4 << 16, b_lbo = (b_mn ? 8192u : 16u) >> 4 << 16;
+          for (; kb < end; ++kb) {
+            if (!ns_wait(&full_bar[stage], phase, args.status, 144, &abort_sh)) {
+              ok = false;
+              break;
             }
-            if constexpr (CG == 2) umma_commit_both(&empty_bar[cur]);
-            else umma_commit(&empty_bar[cur]);
+            tc_fence_after();
+            const int cur = stage;
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+            const uint32_t s0 = (smem_base + cur * C::STAGE_BYTES) >> 4;
+            const uint32_t ad = s0 | a_lbo, bd = (s0 + (one ? 0 : C::OP_BYTES >> 4)) | b_lbo;
+            if (leader) {
+#pragma unroll
+              for (int kk = 0; kk < C::BK / 16; ++kk)
+                ns_mma<CG>(d_tmem, ad + kk * step_a, bd + kk * step_b, desc_hi, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+              if constexpr (CG == 2) umma_commit_both(&empty_bar[cur]);
+              else umma_commit(&empty_bar[cur]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
         if (!ok) break;
         if (leader) {
