@@ -15,6 +15,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <array>
 #include <cmath>
@@ -26,6 +28,8 @@
 
 namespace pb {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr float kXScale = 256.f;   // X is held as 256 X
 constexpr float kAScale = 1024.f;  // A and P as 1024 A, 1024 P
@@ -211,12 +215,14 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ Pa
   }
 }
 
-// ---- small matrices: one block each, fp32 throughout ------------------------------
+// ---- small matrices: one block or cluster each, fp32 throughout -------------------
 // With 32 rows or fewer the products are too small for tensor-core tiles, and rounding to fp16
-// no longer averages out (a 2 x 2 matrix can end 1e-2 off, a 64 x 64 one 1.9e-3).  So one
-// block holds X (fp32; in shared memory, or in ``scratch`` when it does not fit) and runs the
-// whole update in one launch: momentum, norm, every step, and the store.  The block is bound by
-// its own latency: a 5-step 32 x 256 iteration is 15 dependent passes over 32 KB.
+// no longer averages out (a 2 x 2 matrix can end 1e-2 off, a 64 x 64 one 1.9e-3).  So the
+// blocks of one cluster (1 to 8) hold X, each a slice of the long side (fp32; in shared memory,
+// or in ``scratch`` when it does not fit), and run the whole update in one launch: momentum,
+// norm, every step, and the store.  The blocks' partial Gram matrices are added in block order
+// through distributed shared memory; the polynomial is computed by every block for itself.
+// Bound by latency: a 5-step 32 x 256 iteration is 15 dependent passes over 32 KB.
 //   Gram   a warp takes 4 x 4 blocks of row pairs, its lanes run along the long side
 //   apply  a thread takes one column: R values in registers, P from shared memory
 struct SmallArgs {
@@ -225,7 +231,8 @@ struct SmallArgs {
   int nesterov;
   float step;          // step length per unit of learning rate (STEP)
   __nv_bfloat16* dst;  // result [batch][rows][cols] (null: update the parameters)
-  float* scratch;      // [batch][R][ld] (null: shared memory)
+  float* scratch;      // [batch][blocks of a cluster][R][ld] (null: shared memory)
+  int slice;           // long-side elements per block
 };
 constexpr int kSmallRows = 32;
 constexpr int kSmallThreads = 512;
@@ -236,36 +243,56 @@ __global__ void __launch_bounds__(kSmallThreads)
     ns_small_kernel(const __grid_constant__ SmallArgs a, const __grid_constant__ MatTable t,
                     const __grid_constant__ NsStepArgs st) {
   extern __shared__ float small_smem[];
-  __shared__ double red[kSmallThreads / 32];
-  __shared__ float gram[R][R + 1], poly[R][R + 4];
-  const int mat = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+  __shared__ double red[kSmallThreads / 32], norm_part;
+  __shared__ float part[R][R + 1], gram[R][R + 1], poly[R][R + 4];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  const int mat = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
   const bool tall = a.rows > a.cols;
-  const int r = tall ? a.cols : a.rows, c = tall ? a.rows : a.cols, ld = small_ld(c);
-  float* x = a.scratch != nullptr ? a.scratch + static_cast<long>(mat) * R * ld : small_smem;
+  const int r = tall ? a.cols : a.rows, total = tall ? a.rows : a.cols, ld = small_ld(a.slice);
+  const int c0 = min(rank * a.slice, total), c = min(a.slice, total - c0);  // this block's slice
+  float* x = a.scratch != nullptr ? a.scratch + static_cast<long>(blockIdx.x) * R * ld : small_smem;
+  // Element ``e`` of the slice, in memory order: its row of X, its column, its place in the matrix.
+  struct At {
+    int i, j;
+    long k;
+  };
+  auto at = [&](long e) {
+    if (tall) return At{static_cast<int>(e % r), static_cast<int>(e / r), static_cast<long>(c0) * r + e};
+    const int i = static_cast<int>(e / c), j = static_cast<int>(e % c);
+    return At{i, j, static_cast<long>(i) * a.cols + c0 + j};
+  };
+  const long elems = static_cast<long>(r) * c;
   float s = 1.f;
-  if (st.norm != nullptr) {
+  if (st.norm != nullptr) {  // the same for every block of the cluster
     const float n = *st.norm;
     if (!isfinite(n)) return;
     if (a.max_norm > 0.f) s = fminf(1.f, a.max_norm / (n + 1e-6f));
   }
   const TG* gp = static_cast<const TG*>(t.g[mat]);
-  const long numel = static_cast<long>(a.rows) * a.cols;
   double ss = 0.0;
-  for (long e = tid; e < numel; e += kSmallThreads) {
-    float u = load1(gp + e);
+  for (long e = tid; e < elems; e += kSmallThreads) {
+    const At q = at(e);
+    float u = load1(gp + q.k);
     if constexpr (MOM) {
       u *= s;
-      const float m = momentum(u, t.m[mat][e], a.mu);
-      t.m[mat][e] = m;
+      const float m = momentum(u, t.m[mat][q.k], a.mu);
+      t.m[mat][q.k] = m;
       u = a.nesterov ? u + a.mu * (m - u) : m;
     }
     ss += square(u);
-    const int i = static_cast<int>(e / a.cols), j = static_cast<int>(e % a.cols);
-    x[tall ? static_cast<long>(j) * ld + i : static_cast<long>(i) * ld + j] = u;
+    x[static_cast<long>(q.i) * ld + q.j] = u;
   }
   for (int k = tid; k < c; k += kSmallThreads)
     for (int i = r; i < R; ++i) x[static_cast<long>(i) * ld + k] = 0.f;
-  const double inv = 1.0 / (sqrt(block_total(ss, red)) + a.eps);
+  ss = block_total(ss, red);
+  if (blocks > 1) {
+    if (tid == 0) norm_part = ss;
+    cluster.sync();
+    ss = 0.0;
+    for (int b = 0; b < blocks; ++b) ss += *cluster.map_shared_rank(&norm_part, b);
+  }
+  const double inv = 1.0 / (sqrt(ss) + a.eps);
   __syncthreads();
   for (int k = tid; k < c; k += kSmallThreads)
     for (int i = 0; i < r; ++i) x[static_cast<long>(i) * ld + k] = static_cast<float>(x[static_cast<long>(i) * ld + k] * inv);
@@ -295,12 +322,19 @@ __global__ void __launch_bounds__(kSmallThreads)
         for (int j = 0; j < 4; ++j) {
           const float v = warp_sum(acc[i][j]);
           if (lane == 0) {
-            gram[4 * bi + i][4 * bj + j] = v;
-            gram[4 * bj + j][4 * bi + i] = v;
+            part[4 * bi + i][4 * bj + j] = v;
+            part[4 * bj + j][4 * bi + i] = v;
           }
         }
     }
-    __syncthreads();
+    // every block's partial sums are there; and, before any block writes its next ones, read
+    cluster.sync();
+    for (int e = tid; e < R * R; e += kSmallThreads) {
+      float v = 0.f;
+      for (int b = 0; b < blocks; ++b) v += *cluster.map_shared_rank(&part[e / R][e % R], b);
+      gram[e / R][e % R] = v;
+    }
+    cluster.sync();
     for (int e = tid; e < R * R; e += kSmallThreads) {
       const int i = e / R, j = e % R;
       float v = 0.f;
@@ -328,15 +362,16 @@ __global__ void __launch_bounds__(kSmallThreads)
     lr = st.hp != nullptr ? *st.hp : st.lr;
     decay = 1.f - lr * st.weight_decay;
   }
-  for (long e = tid; e < numel; e += kSmallThreads) {
-    const int i = static_cast<int>(e / a.cols), j = static_cast<int>(e % a.cols);
-    const float o = x[tall ? static_cast<long>(j) * ld + i : static_cast<long>(i) * ld + j];
+  const long numel = static_cast<long>(a.rows) * a.cols;
+  for (long e = tid; e < elems; e += kSmallThreads) {
+    const At q = at(e);
+    const float o = x[static_cast<long>(q.i) * ld + q.j];
     if (a.dst != nullptr) {
-      a.dst[mat * numel + e] = __float2bfloat16_rn(o);
+      a.dst[mat * numel + q.k] = __float2bfloat16_rn(o);
     } else {
-      const float w = st.p[mat][e] * decay - lr * a.step * o;
-      st.p[mat][e] = w;
-      if (st.shadow[mat] != nullptr) st.shadow[mat][e] = __float2bfloat16_rn(w);
+      const float w = st.p[mat][q.k] * decay - lr * a.step * o;
+      st.p[mat][q.k] = w;
+      if (st.shadow[mat] != nullptr) st.shadow[mat][q.k] = __float2bfloat16_rn(w);
     }
   }
 }
@@ -671,19 +706,38 @@ bool is_small(int64_t rows, int64_t cols) { return std::min(rows, cols) <= kSmal
 template <int R, typename TG, bool MOM>
 void launch_small(SmallArgs a, const MatTable& t, const NsStepArgs& st, int batch, const at::Tensor& like,
                   cudaStream_t s) {
-  const int64_t ld = small_ld(std::max(a.rows, a.cols));
-  size_t smem = R * ld * sizeof(float);
+  const int64_t side = std::max(a.rows, a.cols);
+  auto bytes = [&](int blocks) { return R * small_ld((side + blocks - 1) / blocks) * sizeof(float); };
+  constexpr size_t kMost = 200 * 1024;
+  // more blocks per matrix while each still has 256 columns and the GPU has room for them, or
+  // until the slices fit in shared memory
+  const int64_t sms = num_sms(like.device().index());
+  int blocks = 1;
+  while (blocks < 8 && side > 256 * blocks && (2 * blocks * batch <= 2 * sms || bytes(blocks) > kMost)) blocks *= 2;
+  a.slice = static_cast<int>((side + blocks - 1) / blocks);
+  size_t smem = bytes(blocks);
   at::Tensor scratch;
-  if (smem > 200 * 1024) {  // a long side beyond shared memory
-    scratch = at::empty({batch * R * ld}, like.options().dtype(at::kFloat));
+  if (smem > kMost) {
+    scratch = at::empty({batch * blocks * static_cast<int64_t>(smem / sizeof(float))}, like.options().dtype(at::kFloat));
     a.scratch = scratch.data_ptr<float>();
     smem = 0;
   }
   auto kern = ns_small_kernel<R, TG, MOM>;
-  if (smem > 40 * 1024)
-    PB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-  kern<<<batch, kSmallThreads, smem, s>>>(a, t, st);
-  PB_CUDA_CHECK(cudaGetLastError());
+  if (smem > 32 * 1024)
+    PB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(batch * blocks, 1, 1);
+  cfg.blockDim = dim3(kSmallThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, t, st));
 }
 
 template <typename TG, bool MOM>

@@ -242,3 +242,17 @@ def test_native_refusals():
             call()
     with pytest.raises(ValueError, match="one device"):
         muon_update_(p, [g[0].cpu()], m, lr=0.1)
+
+
+# rows (or columns) of 32 and fewer go to one cluster per matrix: slices of odd length, more
+# matrices than fit at once, and a long side beyond shared memory
+@pytest.mark.parametrize("batch,m,n", [(1, 32, 3001), (2, 7, 5000), (2, 5000, 31), (40, 16, 2500), (200, 9, 700),
+                                       (1, 5, 60001), (1, 60001, 30), (3, 300, 1)])
+def test_few_rows_and_a_long_side(batch, m, n):
+    x = _rand(batch, m, n, seed=m)
+    x = x * torch.exp(_rand(batch, m, 1, seed=n))  # rows of unequal size
+    assert _off(orthogonalize(x), _exact(x)) <= 2.0**-8 + 1e-4
+    p, g, mom = [0.02 * x], [1e-3 * _rand(batch, m, n, seed=2)], [torch.zeros_like(x)]
+    before = [t.clone() for t in p], [t.clone() for t in mom]
+    muon_update_(p, g, mom, lr=0.02, momentum=0.9, weight_decay=0.1)
+    _check_update(before, g, (p, mom), 0.02, 0.9, 0.1)
