@@ -244,12 +244,14 @@ __global__ void __launch_bounds__(kSmallThreads)
                     const __grid_constant__ NsStepArgs st) {
   extern __shared__ float small_smem[];
   __shared__ double red[kSmallThreads / 32], norm_part;
-  __shared__ float part[R][R + 1], gram[R][R + 1], poly[R][R + 4];
+  __shared__ float part[R][R + 1], gram[R][R + 1];
+  __shared__ __align__(16) float poly[R][R + 4];
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const int mat = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
   const bool tall = a.rows > a.cols;
-  const int r = tall ? a.cols : a.rows, total = tall ? a.rows : a.cols, ld = small_ld(a.slice);
+  const unsigned r = tall ? a.cols : a.rows;
+  const int total = tall ? a.rows : a.cols, ld = small_ld(a.slice);
   const int c0 = min(rank * a.slice, total), c = min(a.slice, total - c0);  // this block's slice
   float* x = a.scratch != nullptr ? a.scratch + static_cast<long>(blockIdx.x) * R * ld : small_smem;
   // Element ``e`` of the slice, in memory order: its row of X, its column, its place in the matrix.
@@ -257,12 +259,12 @@ __global__ void __launch_bounds__(kSmallThreads)
     int i, j;
     long k;
   };
-  auto at = [&](long e) {
+  auto at = [&](unsigned e) {  // 32-bit divisions: the host keeps slices below 2^26 columns
     if (tall) return At{static_cast<int>(e % r), static_cast<int>(e / r), static_cast<long>(c0) * r + e};
-    const int i = static_cast<int>(e / c), j = static_cast<int>(e % c);
+    const int i = static_cast<int>(e / static_cast<unsigned>(c)), j = static_cast<int>(e % static_cast<unsigned>(c));
     return At{i, j, static_cast<long>(i) * a.cols + c0 + j};
   };
-  const long elems = static_cast<long>(r) * c;
+  const unsigned elems = static_cast<unsigned>(r) * c;
   float s = 1.f;
   if (st.norm != nullptr) {  // the same for every block of the cluster
     const float n = *st.norm;
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(kSmallThreads)
   }
   const TG* gp = static_cast<const TG*>(t.g[mat]);
   double ss = 0.0;
-  for (long e = tid; e < elems; e += kSmallThreads) {
+  for (unsigned e = tid; e < elems; e += kSmallThreads) {
     const At q = at(e);
     float u = load1(gp + q.k);
     if constexpr (MOM) {
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kSmallThreads)
     x[static_cast<long>(q.i) * ld + q.j] = u;
   }
   for (int k = tid; k < c; k += kSmallThreads)
-    for (int i = r; i < R; ++i) x[static_cast<long>(i) * ld + k] = 0.f;
+    for (int i = static_cast<int>(r); i < R; ++i) x[static_cast<long>(i) * ld + k] = 0.f;
   ss = block_total(ss, red);
   if (blocks > 1) {
     if (tid == 0) norm_part = ss;
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(kSmallThreads)
   const double inv = 1.0 / (sqrt(ss) + a.eps);
   __syncthreads();
   for (int k = tid; k < c; k += kSmallThreads)
-    for (int i = 0; i < r; ++i) x[static_cast<long>(i) * ld + k] = static_cast<float>(x[static_cast<long>(i) * ld + k] * inv);
+    for (int i = 0; i < static_cast<int>(r); ++i) x[static_cast<long>(i) * ld + k] = static_cast<float>(x[static_cast<long>(i) * ld + k] * inv);
   __syncthreads();
   constexpr int RB = R / 4;
   for (int step = 0; step < a.steps; ++step) {
@@ -328,13 +330,17 @@ __global__ void __launch_bounds__(kSmallThreads)
         }
     }
     // every block's partial sums are there; and, before any block writes its next ones, read
-    cluster.sync();
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
     for (int e = tid; e < R * R; e += kSmallThreads) {
       float v = 0.f;
-      for (int b = 0; b < blocks; ++b) v += *cluster.map_shared_rank(&part[e / R][e % R], b);
+      if (blocks > 1)
+        for (int b = 0; b < blocks; ++b) v += *cluster.map_shared_rank(&part[e / R][e % R], b);
+      else v = part[e / R][e % R];
       gram[e / R][e % R] = v;
     }
-    cluster.sync();
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
     for (int e = tid; e < R * R; e += kSmallThreads) {
       const int i = e / R, j = e % R;
       float v = 0.f;
@@ -349,10 +355,16 @@ __global__ void __launch_bounds__(kSmallThreads)
       for (int i = 0; i < R; ++i) v[i] = x[static_cast<long>(i) * ld + k];
 #pragma unroll 4
       for (int i = 0; i < R; ++i) {
-        float y = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < R; ++j) y += poly[i][j] * v[j];
-        x[static_cast<long>(i) * ld + k] = y;
+        for (int j = 0; j < R; j += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(&poly[i][j]);
+          y.x += w.x * v[j];
+          y.y += w.y * v[j + 1];
+          y.z += w.z * v[j + 2];
+          y.w += w.w * v[j + 3];
+        }
+        x[static_cast<long>(i) * ld + k] = (y.x + y.y) + (y.z + y.w);
       }
     }
     __syncthreads();
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(kSmallThreads)
     decay = 1.f - lr * st.weight_decay;
   }
   const long numel = static_cast<long>(a.rows) * a.cols;
-  for (long e = tid; e < elems; e += kSmallThreads) {
+  for (unsigned e = tid; e < elems; e += kSmallThreads) {
     const At q = at(e);
     const float o = x[static_cast<long>(q.i) * ld + q.j];
     if (a.dst != nullptr) {
@@ -714,6 +726,8 @@ void launch_small(SmallArgs a, const MatTable& t, const NsStepArgs& st, int batc
   const int64_t sms = num_sms(like.device().index());
   int blocks = 1;
   while (blocks < 8 && side > 256 * blocks && (2 * blocks * batch <= 2 * sms || bytes(blocks) > kMost)) blocks *= 2;
+  TORCH_CHECK((side + blocks - 1) / blocks < (1LL << 26), "newton-schulz: ", side, " is too long for a matrix of ",
+              std::min(a.rows, a.cols), " rows");
   a.slice = static_cast<int>((side + blocks - 1) / blocks);
   size_t smem = bytes(blocks);
   at::Tensor scratch;
