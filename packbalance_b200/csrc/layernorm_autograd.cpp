@@ -32,6 +32,7 @@ struct Grads {
 };
 Grads backward_rows(AutogradContext* ctx, const at::Tensor& dy, c10::optional<at::Tensor> dres,
                     c10::optional<at::Tensor> dx_bf16) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "layernorm: its backward pass is not differentiable (create_graph)");
   const auto saved = ctx->get_saved_variables();
   const at::Tensor &x = saved[0], &w = saved[1];
   auto dw = at::empty({x.size(1)}, x.options().dtype(at::kFloat));

@@ -770,12 +770,19 @@ Iteration check_iteration(int64_t steps, const std::vector<double>& coef) {
   return Iteration{(int)steps, (float)coef[0], (float)coef[1], (float)coef[2]};
 }
 
-// Memory that one call writes from several blocks must not be listed twice.
-void check_disjoint(std::vector<std::pair<uintptr_t, uintptr_t>> ranges) {
+// Memory that one call writes must not be listed twice, nor read as a gradient.
+using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
+void check_disjoint(Ranges ranges, const Ranges& reads) {
   std::sort(ranges.begin(), ranges.end());
   for (size_t k = 1; k < ranges.size(); ++k)
     TORCH_CHECK(ranges[k - 1].second <= ranges[k].first,
                 "muon_update: parameters, momenta and shadows must not overlap or be listed twice");
+  for (const auto& r : reads) {
+    const auto next = std::upper_bound(ranges.begin(), ranges.end(), r);
+    TORCH_CHECK((next == ranges.end() || r.second <= next->first) &&
+                    (next == ranges.begin() || std::prev(next)->second <= r.first),
+                "muon_update: gradients must not overlap parameters, momenta or shadows");
+  }
 }
 
 // Cost of one matrix of a shape, to place the longest work first.
@@ -859,10 +866,10 @@ void muon_update(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, 
     __nv_bfloat16* sh;
   };
   std::vector<Mat> mats;
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  auto writes = [&](const at::Tensor& t) {
+  Ranges written, read;
+  auto note = [](Ranges& to, const at::Tensor& t) {
     const auto lo = reinterpret_cast<uintptr_t>(t.data_ptr());
-    if (t.numel() > 0) written.emplace_back(lo, lo + t.numel() * t.element_size());
+    if (t.numel() > 0) to.emplace_back(lo, lo + t.numel() * t.element_size());
   };
   for (size_t k = 0; k < n; ++k) {
     const at::Tensor &p = params[k], &g = grads[k], &m = momenta[k];
@@ -879,10 +886,11 @@ void muon_update(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, 
                       w.numel() == p.numel(),
                   "muon_update: shadow ", k, " must be contiguous bf16 of its parameter's size");
       sh = static_cast<__nv_bfloat16*>(w.data_ptr());
-      writes(w);
+      note(written, w);
     }
-    writes(p);
-    writes(m);
+    note(written, p);
+    note(written, m);
+    note(read, g);
     if (p.numel() == 0) continue;
     Shape& s = by_shape[{rows, cols}];
     s.rows = rows;
@@ -893,7 +901,7 @@ void muon_update(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, 
                       sh == nullptr ? nullptr : sh + i * numel});
     }
   }
-  check_disjoint(written);
+  check_disjoint(std::move(written), read);
   const c10::cuda::CUDAGuard guard(device);
   const int dev = device.index();
   auto s = at::cuda::getCurrentCUDAStream();

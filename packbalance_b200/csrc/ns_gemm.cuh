@@ -450,7 +450,7 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
       // A lane takes the 16-byte piece lane % 8 of rows lane / 8, + 4, + 8, ...; as a piece is
       // used, the one 32 columns on is requested into its registers.  (Holding two blocks ahead
       // spilled, and with 225 KB of shared memory in use a spill's reload comes from L2: 253 us
-      // instead of %STEP% for the 100M model's last product.)
+      // instead of 172 for the 100M model's last product.)
       const int r0 = lane >> 3, q = lane & 7;
       const int rows = (g.M - row0 - r0 + 3) / 4;  // this lane's rows in range
       const long base = static_cast<long>(row0 + r0) * g.N + col0 + 4 * q;
@@ -472,7 +472,7 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
           ns_block_in(s, v);
         }
         float* at = p + base + c;
-        __nv_bfloat16* to = sh + base + c;
+        __nv_bfloat16* to = sh == nullptr ? nullptr : sh + base + c;
         const bool more = c + 32 < W && cols > c + 32;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -488,7 +488,7 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
             if (sh != nullptr) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(w.x, w.y), pack_bf16x2(w.z, w.w));
           }
           at += pitch;
-          to += pitch;
+          if (sh != nullptr) to += pitch;
         }
         __syncwarp();
       }

@@ -72,6 +72,7 @@ STATUS_NAMES = {
     144: "newton-schulz mma: tile copy never landed",
     145: "newton-schulz mma: drain",
     146: "newton-schulz epilogue: accumulator never ready",
+    601: "layernorm: row copy never landed",
     147: "newton-schulz producer: the other CTA's count never came",
 }
 

@@ -203,6 +203,13 @@ def test_other_stream_and_graph_replay():
         _near(dw, ex.dw, ex.dw_tol)
 
 
+def test_second_derivatives_are_refused():
+    x, w, b, dy = _inputs(4, 32, torch.float32)
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(layernorm(x, w, b), x, dy, create_graph=True)
+
+
 def test_native_refusals():
     C = _native.module()
     x, w, b, dy = _inputs(4, 32, torch.float32)

@@ -232,6 +232,8 @@ def test_native_refusals():
         (lambda: muon_update_(p * 2, g * 2, [m[0], m[0].clone()], lr=0.1), "listed twice"),
         (lambda: muon_update_([p[0], both[:128].view(8, 16)], g * 2, [m[0], both[64:192].view(8, 16)], lr=0.1),
          "overlap"),
+        (lambda: muon_update_(p, m, m, lr=0.1), "gradients must not overlap"),
+        (lambda: muon_update_(p, p, m, lr=0.1), "gradients must not overlap"),
         (lambda: muon_update_(p, g, m, lr=0.1, shadows=[p[0].clone()]), "bf16"),
         (lambda: muon_update_(p, g, m, lr=0.1, shadows=[p[0].bfloat16()[:4]]), "size"),
         (lambda: muon_update_(p, g, m, lr=0.1, grad_norm=torch.tensor(1.0), max_norm=1.0), "norm"),
