@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "host_utils.h"
@@ -350,7 +351,9 @@ __global__ void __launch_bounds__(ln_threads(T))
   const float inv_n = 1.f / n;
   __shared__ __align__(16) float red[G][4 * (T / 32)];
   extern __shared__ __align__(16) uint8_t ring_smem[];
-  float* cols = reinterpret_cast<float*>(ring_smem);  // [2][T * K * V] after the last row (G > 1)
+  // [2][T * K * V] after the last row (G > 1), in the slots' memory; not over the ring's mbarriers,
+  // whose memory may not be used otherwise while they are valid
+  float* cols = reinterpret_cast<float*>(ring_smem + (RING ? (G * slots * 8 + 15) & ~15 : 0));
   const int t = threadIdx.x % T, grp = threadIdx.x / T;
   int flip = 0;
   const long stride = static_cast<long>(gridDim.x) * G;
@@ -724,15 +727,20 @@ RowLaunch row_launch(int threads, int groups, int64_t row_bytes, size_t least, i
     const int64_t room = std::min(kRingBytes * (threads / 256), kRingMost - 64);
     l.slots = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, room / one)));
     TORCH_CHECK(l.slots * one <= kRingMost - 64, "layernorm: row of ", row_bytes, " bytes does not fit");
-    l.smem = std::max(least, static_cast<size_t>(groups * l.slots * row_bytes + (groups * l.slots * 8 + 15) / 16 * 16));
+    l.smem = std::max(least, static_cast<size_t>(groups * l.slots * row_bytes)) + (groups * l.slots * 8 + 15) / 16 * 16;
   }
   static int most[64] = {0};  // of this kernel
   if (l.smem > 48 * 1024 && most[dev] == 0) {
     PB_CUDA_CHECK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost));
     most[dev] = 1;
   }
-  int n = 0;
-  PB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, threads, l.smem));
+  // resident blocks at the shared-memory size last asked for (the query costs as much as a launch)
+  thread_local std::pair<size_t, int> resident[64] = {};
+  int& n = resident[dev].second;
+  if (n == 0 || resident[dev].first != l.smem) {
+    resident[dev].first = l.smem;
+    PB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, threads, l.smem));
+  }
   l.blocks = static_cast<int>(std::min<int64_t>((rows + groups - 1) / groups,
                                                 static_cast<int64_t>(std::max(1, n)) * num_sms(dev)));
   return l;

@@ -105,6 +105,33 @@ def test_add_forward_and_gradients(rows, n):
     _near(db, ex.db, ex.db_tol)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n", [(9001, 128), (8192, 256), (8192, 512), (8192, 768), (4097, 1408), (3000, 2048),
+                                    (2500, 4096), (1500, 8192), (400, 16384), (6000, 257), (3000, 1409)])
+def test_many_rows_per_block(rows, n, dtype):
+    """Every slot of the row ring is filled several times; every type of dy, with and without a
+    residual gradient; the memory the calls get holds NaN beforehand."""
+    C = _native.module()
+    x, w, b, dy = _inputs(rows, n, dtype, seed=n)
+    _, y, mean, rstd = C.add_layernorm_fwd(x, None, w, b, 1e-5, False)
+    dres = torch.randn(rows, n, device=dev) if dtype == torch.float32 else None
+    for g, res in ((dy, None), (dy, dres), (dy.bfloat16(), dres), (dy.bfloat16(), None)):
+        if res is None and dtype == torch.float32 and g.dtype == torch.bfloat16:
+            continue
+        ex = _Exact(x, w, b, 1e-5, g, res)
+        _near(y, ex.y, ex.y_tol)
+        copy = torch.empty(rows, n, device=dev, dtype=torch.bfloat16) if dtype == torch.float32 else None
+        for _ in range(4):
+            torch.full((2 * 512 * n,), float("nan"), device=dev)
+            dw, db = torch.empty(n, device=dev), torch.empty(n, device=dev)
+            dx = C.layernorm_bwd(g, x, w, mean, rstd, res, copy, dw, db, False)
+            _near(dw, ex.dw, ex.dw_tol)
+            _near(db, ex.db, ex.db_tol)
+        _near(dx, ex.dx, ex.dx_tol)
+        if copy is not None:
+            assert torch.equal(copy, dx.bfloat16())
+
+
 def test_unused_sum_output_has_zero_gradient():
     x, w, b, _ = _inputs(12, 96, torch.float32)
     delta = torch.zeros(12, 96, device=dev, dtype=torch.bfloat16)
