@@ -10,7 +10,8 @@
 // rounding, so pass 1 updates the momentum and sums u^2 per 8192-element chunk, and pass 2
 // reads momentum and gradient again, adds up its matrix's chunk sums (in chunk order: no
 // atomics, the result does not depend on scheduling) and writes X0 as fp16 and e4m3 low parts.
-// Both are memory-bound.  The products follow as three launches per step (ns_gemm.cuh).
+// Both are memory-bound (85M elements: 137 and 135 us, 7.4 TB/s and 6.9 TB/s).  The products follow
+// as three launches per step (ns_gemm.cuh).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -31,6 +31,10 @@
 // the operand is MN-major.  So symmetry halves the stores as well as the products.
 //   warp 0 TMA producer, warp 1 TMEM allocation and MMA issue, warps 2-9 epilogue: two per
 //   quarter of the TMEM lanes, each finishing half of the tile's columns.
+//
+// Measured (B200, the 100M model's 84 matrices): GRAM 57 us (0.95 PFLOP/s of useful work), POLY
+// 45 us (K = 768 or less: epilogue and pipeline start), APPLY 97 us, 142 us where it reads and
+// writes low parts (HBM), STEP 172 us (HBM: 850 MB at 4.9 TB/s).
 #pragma once
 
 #include <cuda_fp16.h>
