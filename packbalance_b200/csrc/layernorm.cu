@@ -730,7 +730,8 @@ RowLaunch row_launch(int threads, int groups, int64_t row_bytes, size_t least, i
     l.smem = std::max(least, static_cast<size_t>(groups * l.slots * row_bytes)) + (groups * l.slots * 8 + 15) / 16 * 16;
   }
   static int most[64] = {0};  // of this kernel
-  if (l.smem > 48 * 1024 && most[dev] == 0) {
+  // 48 KB need no opt-in, but they include the kernel's static arrays (at most 512 bytes)
+  if (l.smem > 47 * 1024 && most[dev] == 0) {
     PB_CUDA_CHECK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost));
     most[dev] = 1;
   }
