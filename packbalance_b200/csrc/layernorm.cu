@@ -4,9 +4,12 @@
 //   dx = r (g - mean(g) - xh mean(g xh)) [+ dres],  g = dy w
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
-// The variance is taken around the row's own mean (a second pass over the row), so a row
-// with a large common offset loses nothing.  Statistics, sums and gradients are fp32; only
-// the stored activations are rounded to the caller's type.  Every sum has a fixed order (no
+// The mean is the unevaluated sum of two floats: the sum of the row over n, and the mean of the
+// differences d from that, which the second pass over the row adds up beside d^2.  A row whose
+// offset is far larger than its spread has a first part that is off by a few of its own last
+// places, and at an offset of 1e4 one of those is 1e-3; the second part takes that out again.
+// Statistics, sums and gradients are fp32; only the stored activations are rounded to the
+// caller's type.  Every sum has a fixed order (no
 // atomics), so two runs on the same inputs agree bit for bit.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -125,6 +128,13 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, const float* v) {
                                               pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
+// 1 / sqrt(var + eps) from the mean square of the differences from a mean that is off by ``dmu``.
+// (The rounded difference may be below zero; NaN stays.)
+__device__ __forceinline__ float rstd_of(float msq, float dmu, float eps) {
+  const float var = fmaf(-dmu, dmu, msq);
+  return rsqrtf((var < 0.f ? 0.f : var) + eps);
+}
+
 constexpr int ln_threads(int t) { return t < 256 ? 256 : t; }
 
 // Sums of N (1 or 2) values over the T threads of a row, in a fixed order; every thread gets them.
@@ -208,7 +218,7 @@ __global__ void __launch_bounds__(ln_threads(T))
   constexpr bool RING = V > 1;
   constexpr int P = K * V / 2;  // pairs
   const float inv_n = 1.f / n;
-  __shared__ __align__(16) float red[G][2 * (T / 32)];
+  __shared__ __align__(16) float red[G][4 * (T / 32)];
   extern __shared__ __align__(16) uint8_t ring_smem[];
   const int t = threadIdx.x % T, grp = threadIdx.x / T;
   int flip = 0;
@@ -301,6 +311,7 @@ __global__ void __launch_bounds__(ln_threads(T))
     const float mu = s[0] * inv_n;
     const f2 minus = mk2(-mu, -mu);
     acc = mk2(0.f, 0.f);
+    f2 rest = mk2(0.f, 0.f);  // what the mean so far leaves
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       v[i] = add2(v[i], minus);
@@ -310,23 +321,27 @@ __global__ void __launch_bounds__(ln_threads(T))
         if (split && ((2 * i + 1) * T + t) >= n) {
           const float a = un2(v[i]).x;
           acc = fma2(mk2(a, 0.f), mk2(a, 0.f), acc);
+          rest = add2(rest, mk2(a, 0.f));
         } else {
           acc = fma2(v[i], v[i], acc);
+          rest = add2(rest, v[i]);
         }
       }
     }
-    s[0] = sum2(acc);
-    row_sums<T>(s, red[grp], flip);
-    const float r = rsqrtf(s[0] * inv_n + eps);
+    float s2[2] = {sum2(rest), sum2(acc)};
+    row_sums<T>(s2, red[grp], flip);
+    const float dmu = s2[0] * inv_n;
+    const float r = rstd_of(s2[1] * inv_n, dmu, eps);
     if (t == 0 && mean != nullptr) {
-      mean[row] = mu;
+      mean[2 * row] = mu;
+      mean[2 * row + 1] = dmu;
       rstd[row] = r;
     }
-    const f2 r2 = mk2(r, r);
+    const f2 r2 = mk2(r, r), dr = mk2(-dmu * r, -dmu * r);
     float o[K * V];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const float2 q = un2(fma2(mul2(v[i], r2), wv[i], bv[i]));
+      const float2 q = un2(fma2(fma2(v[i], r2, dr), wv[i], bv[i]));
       o[2 * i] = q.x;
       o[2 * i + 1] = q.y;
     }
@@ -403,14 +418,15 @@ __global__ void __launch_bounds__(ln_threads(T))
       }
     }
   };
-  float mu_n = 0.f, r_n = 0.f;
+  float mu_n = 0.f, dmu_n = 0.f, r_n = 0.f;
   if (row < rows) {
-    mu_n = mean[row];
+    mu_n = mean[2 * row];
+    dmu_n = mean[2 * row + 1];
     r_n = rstd[row];
     if (!RING) fetch(x + row * n, dy + row * n, dres + row * n);
   }
   for (; row < rows; row += stride) {
-    const float mu = mu_n, r = r_n;
+    const float mu = mu_n, r = r_n, dmu_r = -dmu_n * r_n;
     if constexpr (RING) {
       ring.wait(status);
       const uint8_t* q = ring.row();
@@ -419,14 +435,15 @@ __global__ void __launch_bounds__(ln_threads(T))
     }
     const long after = row + stride;
     if (after < rows) {
-      mu_n = mean[after];
+      mu_n = mean[2 * after];
+      dmu_n = mean[2 * after + 1];
       r_n = rstd[after];
     }
     f2 xh[P], g[P];
     float res[RES ? K * V : 1];
     f2 a1 = mk2(0.f, 0.f), a2 = mk2(0.f, 0.f);
     {
-      const f2 r2 = mk2(r, r);
+      const f2 r2 = mk2(r, r), dr = mk2(dmu_r, dmu_r);
       float u[K * V], q[K * V];
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -445,9 +462,9 @@ __global__ void __launch_bounds__(ln_threads(T))
       if (!RING && after < rows) fetch(x + after * n, dy + after * n, dres + after * n);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        // (x - mu) r, the difference rounded first: x r - mu r would lose a row's common offset
+        // (x - mu) r - dmu r, the difference rounded first: x r - mu r would lose a row's common offset
         const f2 d = add2(mk2(u[2 * i], u[2 * i + 1]), mk2(-mu, -mu));
-        xh[i] = mul2(d, r2);
+        xh[i] = fma2(d, r2, dr);
         g[i] = mk2(q[2 * i], q[2 * i + 1]);
         const f2 t2 = mul2(g[i], xh[i]);
         aw[i] = add2(aw[i], t2);
@@ -585,17 +602,21 @@ __global__ void ln_fwd_kernel(const TI* __restrict__ xp, const __nv_bfloat16* __
   }
   const float mu = block_sum(s, red) / n;
   float ss = 0.f;
+  s = 0.f;
   for (int c = threadIdx.x; c < n; c += blockDim.x) {
     const float d = value(c) - mu;
+    s += d;
     ss += d * d;
   }
-  const float r = rsqrtf(block_sum(ss, red) / n + eps);
+  const float dmu = block_sum(s, red) / n;
+  const float r = rstd_of(block_sum(ss, red) / n, dmu, eps);
   if (threadIdx.x == 0 && mean != nullptr) {
-    mean[row] = mu;
+    mean[2 * row] = mu;
+    mean[2 * row + 1] = dmu;
     rstd[row] = r;
   }
   for (int c = threadIdx.x; c < n; c += blockDim.x)
-    stf(y + off + c, (value(c) - mu) * r * w[c] + (b != nullptr ? b[c] : 0.f));
+    stf(y + off + c, ((value(c) - mu) - dmu) * r * w[c] + (b != nullptr ? b[c] : 0.f));
 }
 
 template <typename TI, typename TD>
@@ -606,18 +627,18 @@ __global__ void ln_bwd_dx_kernel(const TD* __restrict__ dy, const TI* __restrict
   __shared__ float red[32];
   const long row = blockIdx.x;
   const long off = row * n;
-  const float mu = mean[row], r = rstd[row];
+  const float mu = mean[2 * row], dmu = mean[2 * row + 1], r = rstd[row];
   float s1 = 0.f, s2 = 0.f;
   for (int c = threadIdx.x; c < n; c += blockDim.x) {
     const float g = ldf(dy + off + c) * w[c];
     s1 += g;
-    s2 += g * ((ldf(x + off + c) - mu) * r);
+    s2 += g * (((ldf(x + off + c) - mu) - dmu) * r);
   }
   s1 = block_sum(s1, red) / n;
   s2 = block_sum(s2, red) / n;
   for (int c = threadIdx.x; c < n; c += blockDim.x) {
     const float g = ldf(dy + off + c) * w[c];
-    const float xh = (ldf(x + off + c) - mu) * r;
+    const float xh = ((ldf(x + off + c) - mu) - dmu) * r;
     float d = r * (g - s1 - xh * s2);
     if (dres != nullptr) d += dres[off + c];
     stf(dx + off + c, d);
@@ -638,7 +659,7 @@ __global__ void ln_bwd_dw_kernel(const TD* __restrict__ dy, const TI* __restrict
     for (int row = wid; row < rows; row += 8) {
       const long at = static_cast<long>(row) * n + c;
       const float d = ldf(dy + at);
-      sw += d * ((ldf(x + at) - mean[row]) * rstd[row]);
+      sw += d * (((ldf(x + at) - mean[2L * row]) - mean[2L * row + 1]) * rstd[row]);
       sb += d;
     }
   }
@@ -752,7 +773,8 @@ bool aligned(const at::Tensor& t, size_t bytes) { return reinterpret_cast<uintpt
 }  // namespace
 
 // x [rows, n] fp32 or bf16, ``delta`` (bf16, with an fp32 x): the row is x + delta, returned
-// as the first tensor.  -> {x + delta or x, y, mean, rstd}; the statistics only if ``stats``.
+// as the first tensor.  -> {x + delta or x, y, mean [rows, 2], rstd [rows]}: the row's mean is the sum
+// of its two floats.  The statistics only if ``stats``.
 std::vector<at::Tensor> add_layernorm_fwd(at::Tensor x, c10::optional<at::Tensor> delta, at::Tensor w,
                                           c10::optional<at::Tensor> b, double eps, bool out_bf16, bool stats) {
   TORCH_CHECK(x.dim() == 2 && x.size(1) > 0, "layernorm: x must be [rows, n] with n > 0");
@@ -774,7 +796,7 @@ std::vector<at::Tensor> add_layernorm_fwd(at::Tensor x, c10::optional<at::Tensor
   auto y = at::empty(x.sizes(), x.options().dtype(out_bf16 ? at::kBFloat16 : x.scalar_type()));
   at::Tensor mean, rstd;
   if (stats) {
-    mean = at::empty({rows}, x.options().dtype(at::kFloat));
+    mean = at::empty({rows, 2}, x.options().dtype(at::kFloat));
     rstd = at::empty({rows}, x.options().dtype(at::kFloat));
   }
   if (rows == 0) return {xo, y, mean, rstd};
@@ -837,7 +859,7 @@ at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor m
   const int64_t rows = x.size(0), n = x.size(1);
   TORCH_CHECK(rows < (1LL << 31) && n < (1LL << 31), "layernorm: rows and n must fit 32 bits");
   check_vec(w, n, x, "weight");
-  check_vec(mean, rows, x, "mean");
+  check_vec(mean, 2 * rows, x, "mean");
   check_vec(rstd, rows, x, "rstd");
   check_vec(dw_out, n, x, "dw_out");
   if (db_out.has_value()) check_vec(*db_out, n, x, "db_out");
