@@ -1,4 +1,5 @@
-"""Native layer normalisation of rows whose mean is far larger than their spread.
+"""Native layer normalisation of rows whose mean is far larger than their spread, and of gradients
+whose sums are known.
 
 Bounds, with u = 2^-24.  Up to 16384 columns a thread adds at most 16 elements, then 10 levels of
 shuffles and warps' sums follow, so a row's sum passes fewer than D = 40 roundings whatever its width;
@@ -12,6 +13,7 @@ column's sum passes at most rows / 148 roundings in a thread and 100 more where 
 import pytest
 import torch
 
+from packbalance_b200.ops import _native
 from packbalance_b200.ops.layernorm import add_layernorm, layernorm
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +100,43 @@ def test_sums_far_from_zero(n):
                            (db, ex.db, ex.db_tol)):
         _near(got, want, tol)
     assert torch.equal(dd, dx.bfloat16())
+TALL = [(9001, 128), (8192, 256), (8192, 768), (4097, 1408), (2500, 4096), (1500, 8192), (400, 16384), (6000, 257),
+          (3000, 1409), (700, 20001)]
+
+
+def _plain_rows(rows, n, dtype):
+    gen = torch.Generator(device=dev).manual_seed(n)
+    x = torch.randn(rows, n, generator=gen, device=dev) + 0.5
+    return x.to(dtype), 1 + 0.2 * torch.randn(n, generator=gen, device=dev), torch.zeros(n, device=dev), gen
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n", TALL)
+def test_column_sums(rows, n, dtype):
+    C = _native.module()
+    x, w, b, gen = _plain_rows(rows, n, dtype)
+    _, y, mean, rstd = C.add_layernorm_fwd(x, None, w, b, 1e-5, False)
+
+    def grads(dy):
+        dw, db = torch.full((n,), float("nan"), device=dev), torch.full((n,), float("nan"), device=dev)
+        dx = C.layernorm_bwd(dy, x, w, mean, rstd, None, None, dw, db, False)
+        return dx, dw, db
+
+    # whole numbers of 4 bits: every partial sum is exact
+    dy = torch.randint(-8, 9, (rows, n), generator=gen, device=dev).to(dtype)
+    dx, dw, db = grads(dy)
+    ex = _Exact(x, w, b, 1e-5, dy)
+    assert torch.equal(db.double(), ex.db)
+    _near(dw, ex.dw, ex.dw_tol)
+    _near(dx, ex.dx, ex.dx_tol)
+    # a gradient in one row alone: the sums are that row's terms
+    for at in {0, 1, rows // 2 + 3, rows - 148, rows - 7, rows - 2, rows - 1}:
+        dy = torch.zeros(rows, n, device=dev, dtype=dtype)
+        dy[at] = torch.randn(n, generator=gen, device=dev).to(dtype)
+        dx, dw, db = grads(dy)
+        one = _Exact(x[at : at + 1], w, b, 1e-5, dy[at : at + 1])
+        assert torch.equal(db, dy[at].float())
+        _near(dw, one.dw, one.dw_tol)
+        _near(dx[at : at + 1], one.dx, one.dx_tol)
+        dx[at] = 0
+        assert not dx.any()
