@@ -24,6 +24,14 @@ at::Tensor param_of(const at::Tensor& w) { return w.to(at::kFloat).contiguous();
 c10::optional<at::Tensor> param_of(const c10::optional<at::Tensor>& b) {
   return b.has_value() ? c10::optional<at::Tensor>(param_of(*b)) : c10::nullopt;
 }
+// Tangents of forward-mode differentiation would be dropped: the kernels work on raw memory, and
+// whether a node is made depends on the backward pass alone.
+void refuse_tangent(const at::Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "layernorm: forward-mode derivatives are not available on CUDA");
+}
+void refuse_tangent(const c10::optional<at::Tensor>& t) {
+  if (t.has_value()) refuse_tangent(*t);
+}
 bool wants_grad(const at::Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
@@ -84,6 +92,9 @@ struct AddLayerNormFn : torch::autograd::Function<AddLayerNormFn> {
 
 // Public forms (arguments already checked): a node only where a gradient is wanted.
 at::Tensor layernorm(at::Tensor x, at::Tensor w, c10::optional<at::Tensor> b, double eps) {
+  refuse_tangent(x);
+  refuse_tangent(w);
+  refuse_tangent(b);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return LayerNormFn::apply(x, w, b, eps);
   at::NoGradGuard guard;
@@ -93,6 +104,10 @@ at::Tensor layernorm(at::Tensor x, at::Tensor w, c10::optional<at::Tensor> b, do
 
 std::vector<at::Tensor> add_layernorm(at::Tensor x, at::Tensor delta, at::Tensor w, c10::optional<at::Tensor> b,
                                       double eps) {
+  refuse_tangent(x);
+  refuse_tangent(delta);
+  refuse_tangent(w);
+  refuse_tangent(b);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(delta) || wants_grad(w) || wants_grad(b)))
     return AddLayerNormFn::apply(x, delta, w, b, eps);
   at::NoGradGuard guard;

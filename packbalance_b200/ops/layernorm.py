@@ -36,7 +36,8 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
               eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, in ``x``'s
     type (fp32 or bf16; any width, any leading shape).  ``weight`` and ``bias`` (optional)
-    are vectors of that width; their gradients are sums over all rows in fp32."""
+    are vectors of that width; their gradients are sums over all rows in fp32.  On CUDA there
+    are first derivatives by a backward pass only: forward mode and ``create_graph`` are errors."""
     _check(x, weight, bias, "layernorm")
     if not x.is_cuda:
         return layernorm_reference(x, weight, bias, eps)
