@@ -20,6 +20,11 @@ at::Tensor rows_of(const at::Tensor& t, int64_t n) {
   if (t.dim() == 2 && t.is_contiguous()) return t;
   return t.reshape({-1, n}).contiguous();
 }
+// A result in its caller's shape.  Not a view for autograd: torch refuses to change a view that a
+// node returned in place.
+at::Tensor shaped(const at::Tensor& t, const at::Tensor& like) {
+  return t.dim() == like.dim() ? t : at::_unsafe_view(t, like.sizes());
+}
 at::Tensor param_of(const at::Tensor& w) { return w.to(at::kFloat).contiguous(); }
 c10::optional<at::Tensor> param_of(const c10::optional<at::Tensor>& b) {
   return b.has_value() ? c10::optional<at::Tensor>(param_of(*b)) : c10::nullopt;
@@ -42,7 +47,7 @@ Grads backward_rows(AutogradContext* ctx, const at::Tensor& dy, c10::optional<at
                     c10::optional<at::Tensor> dx_bf16) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "layernorm: its backward pass is not differentiable (create_graph)");
   const auto saved = ctx->get_saved_variables();
-  const at::Tensor &x = saved[0], &w = saved[1];
+  const at::Tensor x = rows_of(saved[0], saved[0].size(-1)), &w = saved[1];
   auto dw = at::empty({x.size(1)}, x.options().dtype(at::kFloat));
   c10::optional<at::Tensor> db;
   const int64_t bias_type = ctx->saved_data["bias_type"].toInt();
@@ -62,7 +67,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     auto x2 = rows_of(x, x.size(-1));
     auto r = add_layernorm_fwd(x2, c10::nullopt, param_of(w), param_of(b), eps, false, true);
     save(ctx, x2, w, b, r[2], r[3]);
-    return r[1].view(x.sizes());
+    return shaped(r[1], x);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const at::Tensor& dy = grads[0];
@@ -76,8 +81,10 @@ struct AddLayerNormFn : torch::autograd::Function<AddLayerNormFn> {
                                const c10::optional<at::Tensor>& b, double eps) {
     const int64_t n = x.size(-1);
     auto r = add_layernorm_fwd(rows_of(x, n), rows_of(delta, n), param_of(w), param_of(b), eps, true, true);
-    save(ctx, r[0], w, b, r[2], r[3]);
-    return {r[0].view(x.sizes()), r[1].view(x.sizes())};
+    // saved as it is returned, so that a change in place is noticed by the backward pass
+    auto total = shaped(r[0], x);
+    save(ctx, total, w, b, r[2], r[3]);
+    return {total, shaped(r[1], x)};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const at::Tensor &dtotal = grads[0], &dy = grads[1];
@@ -98,8 +105,8 @@ at::Tensor layernorm(at::Tensor x, at::Tensor w, c10::optional<at::Tensor> b, do
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return LayerNormFn::apply(x, w, b, eps);
   at::NoGradGuard guard;
-  return add_layernorm_fwd(rows_of(x, x.size(-1)), c10::nullopt, param_of(w), param_of(b), eps, false, false)[1].view(
-      x.sizes());
+  return shaped(add_layernorm_fwd(rows_of(x, x.size(-1)), c10::nullopt, param_of(w), param_of(b), eps, false, false)[1],
+                x);
 }
 
 std::vector<at::Tensor> add_layernorm(at::Tensor x, at::Tensor delta, at::Tensor w, c10::optional<at::Tensor> b,
@@ -113,7 +120,7 @@ std::vector<at::Tensor> add_layernorm(at::Tensor x, at::Tensor delta, at::Tensor
   at::NoGradGuard guard;
   const int64_t n = x.size(-1);
   auto r = add_layernorm_fwd(rows_of(x, n), rows_of(delta, n), param_of(w), param_of(b), eps, true, false);
-  return {r[0].view(x.sizes()), r[1].view(x.sizes())};
+  return {shaped(r[0], x), shaped(r[1], x)};
 }
 
 }  // namespace pb

@@ -47,7 +47,8 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
 def add_layernorm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
                   eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
     """``(x + delta, layernorm(x + delta))`` for an fp32 residual stream ``x`` and a bf16
-    ``delta`` of the same shape; the sum is fp32, the normalised rows are bf16."""
+    ``delta`` of the same shape; the sum is fp32, the normalised rows are bf16.  The
+    backward pass reads the sum, so change that in place only where none follows."""
     _check(x, weight, bias, "add_layernorm")
     if x.dtype != torch.float32 or delta.dtype != torch.bfloat16 or delta.shape != x.shape:
         raise ValueError("add_layernorm: fp32 x and bf16 delta of the same shape, got "
