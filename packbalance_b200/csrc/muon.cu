@@ -9,7 +9,7 @@
 // Two passes over the inputs come first: the norm has to be known before the first fp16
 // rounding, so pass 1 updates the momentum and sums u^2 per 8192-element chunk, and pass 2
 // reads momentum and gradient again, adds up its matrix's chunk sums (in chunk order: no
-// atomics, the result does not depend on scheduling) and writes X0 as fp16 and e4m3 low parts.
+// atomics, the result does not depend on scheduling) and writes X0 as fp16 high and low parts.
 // Both are memory-bound (85M elements: 137 and 135 us, 7.4 TB/s and 6.9 TB/s).  The products follow
 // as three launches per step (ns_gemm.cuh).
 #include <ATen/ATen.h>
@@ -44,14 +44,13 @@ struct MatTable {
 struct PassGroup {
   int mat0, batch;       // matrices [mat0, mat0 + batch) of the table
   int rows, cols, ld;    // ld: padded row length of X
-  int low_ld;            // and of its low part
   long numel;            // rows * cols
   int chunks;            // chunks per matrix
   int block_end;         // running total of blocks
   int part0;             // index of the group's first partial sum
   int vec;               // 4-element accesses allowed
-  __half* hi;            // X0 [batch][rows][ld] and its low part [batch][rows][low_ld]
-  uint8_t* low;
+  __half* hi;            // X0 [batch][rows][ld] and its low part (null: none)
+  __half* low;
 };
 struct PassArgs {
   PassGroup g[kNsGroups];
@@ -157,7 +156,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Pa
   if (threadIdx.x == 0) a.part[g.part0 + local] = ss;
 }
 
-// Pass 2: X0 = u / (|u| + eps) as fp16 with e4m3 low parts.
+// Pass 2: X0 = u / (|u| + eps) as fp16 high and low parts.
 template <typename TG, bool MOM>
 __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ PassArgs a,
                                                        const __grid_constant__ MatTable t) {
@@ -176,7 +175,6 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ Pa
   const TG* gp = static_cast<const TG*>(t.g[g.mat0 + mat]);
   const float* mp = MOM ? t.m[g.mat0 + mat] : nullptr;
   const long base = static_cast<long>(mat) * g.rows * g.ld;
-  const long lbase = static_cast<long>(mat) * g.rows * g.low_ld;
   if (g.vec) {
 #pragma unroll 4
     for (long i = lo + threadIdx.x * 4; i < hi; i += 1024) {
@@ -195,10 +193,9 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ Pa
       if (g.low != nullptr) {
         const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
         const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-        const long to = lbase + (g.low_ld == g.cols ? i : i / g.cols * g.low_ld + i % g.cols);
-        *reinterpret_cast<uint32_t*>(g.low + to) =
-            pack_low2((u.x - h0.x) * kNsLowScale, (u.y - h0.y) * kNsLowScale) |
-            pack_low2((u.z - h1.x) * kNsLowScale, (u.w - h1.y) * kNsLowScale) << 16;
+        *reinterpret_cast<uint2*>(g.low + at) =
+            make_uint2(pack_f16x2((u.x - h0.x) * kNsLowScale, (u.y - h0.y) * kNsLowScale),
+                       pack_f16x2((u.z - h1.x) * kNsLowScale, (u.w - h1.y) * kNsLowScale));
       }
     }
   } else {
@@ -209,9 +206,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ Pa
       const long at = base + i / g.cols * g.ld + i % g.cols;
       const __half h = __float2half_rn(u);
       g.hi[at] = h;
-      if (g.low != nullptr)
-        g.low[lbase + i / g.cols * g.low_ld + i % g.cols] =
-            static_cast<uint8_t>(pack_low2((u - __half2float(h)) * kNsLowScale, 0.f));
+      if (g.low != nullptr) g.low[at] = __float2half_rn((u - __half2float(h)) * kNsLowScale);
     }
   }
 }
@@ -440,11 +435,11 @@ __global__ void __launch_bounds__(256) adamw_ranges_kernel(
 }
 
 // ------------------------------------ host ----------------------------------------
-CUtensorMap map3(const void* ptr, CUtensorMapDataType type, int bytes, int64_t cols, int64_t rows, int64_t batch, int64_t ld,
+CUtensorMap map3(const void* ptr, CUtensorMapDataType type, int64_t cols, int64_t rows, int64_t batch, int64_t ld,
                  uint32_t box, CUtensorMapSwizzle swizzle) {
   CUtensorMap m;
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
-  cuuint64_t strides[2] = {(cuuint64_t)(ld * bytes), (cuuint64_t)(rows * ld * bytes)};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(rows * ld) * 2};
   cuuint32_t boxes[3] = {box, box, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = tmap_encoder()(&m, type, 3, const_cast<void*>(ptr), dims, strides, boxes, estr,
@@ -455,10 +450,10 @@ CUtensorMap map3(const void* ptr, CUtensorMapDataType type, int bytes, int64_t c
   return m;
 }
 CUtensorMap load_map(const __half* p, int64_t cols, int64_t rows, int64_t batch, int64_t ld) {
-  return map3(p, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, cols, rows, batch, ld, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  return map3(p, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, cols, rows, batch, ld, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 CUtensorMap store_map(const void* p, int64_t cols, int64_t rows, int64_t batch, int64_t ld, bool bf16) {
-  return map3(p, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, cols, rows, batch, ld, 32,
+  return map3(p, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, cols, rows, batch, ld, 32,
               CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
@@ -471,9 +466,7 @@ struct Shape {
   int64_t ld() const { return (cols + 7) / 8 * 8; }
   int64_t ldr() const { return (r() + 7) / 8 * 8; }
   bool tall() const { return rows > cols; }
-  int64_t low_ld() const { return (cols + 15) / 16 * 16; }
-  __half *x[2] = {nullptr, nullptr}, *gram = nullptr, *poly = nullptr;
-  uint8_t* low = nullptr;
+  __half *x[2] = {nullptr, nullptr}, *low = nullptr, *gram = nullptr, *poly = nullptr;
 };
 
 template <int CG, int MODE, class Step>
@@ -601,11 +594,9 @@ void ns_iterate(std::vector<Shape>& shapes, const Iteration& it, int dev, cudaSt
     y.M = (int)sh.rows;
     y.N = (int)sh.cols;
     y.K = (int)r;
-    y.add_batch = sh.rows * sh.low_ld();
-    y.add_ld = (int)sh.low_ld();
-    if (it.steps > 3)
-      y.low = map3(sh.low, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, sh.cols, sh.rows, B, sh.low_ld(), 32,
-                   CU_TENSOR_MAP_SWIZZLE_NONE);
+    y.add_batch = sh.rows * sh.ld();
+    y.add_ld = (int)sh.ld();
+    if (it.steps > 3) y.low = store_map(sh.low, sh.cols, sh.rows, B, sh.ld(), false);
     for (NsGroup* p : {&g, &q, &y}) p->k_blocks = (p->K + 63) / 64;
   }
   for (int step = 0, cur = 0; step < it.steps; ++step, cur ^= 1) {
@@ -615,7 +606,7 @@ void ns_iterate(std::vector<Shape>& shapes, const Iteration& it, int dev, cudaSt
       NsGroup& y = apply.g[k];
       (shapes[k].tall() ? y.a : y.b) = x_load[k][cur];
       // the input carries a low part while at least two steps follow this one
-      y.low_in = step + 2 < it.steps ? shapes[k].low : nullptr;
+      y.add = step + 2 < it.steps ? shapes[k].low : nullptr;
       y.store_low = step + 3 < it.steps;
       if (!final) y.out = x_store[k][cur ^ 1];
     }
@@ -642,8 +633,8 @@ at::Tensor make_workspace(std::vector<Shape>& shapes, const Iteration& it, int64
   std::vector<std::array<int64_t, 5>> at(shapes.size());
   for (size_t k = 0; k < shapes.size(); ++k) {
     const Shape& s = shapes[k];
-    const int64_t xb = s.batch() * s.rows * s.ld() * 2, lb = s.batch() * s.rows * s.low_ld(), ab = s.batch() * s.r() * s.ldr() * 2;
-    at[k] = {take(xb), it.steps > 1 ? take(xb) : 0, it.steps > 2 ? take(lb) : -1, take(ab), take(ab)};
+    const int64_t xb = s.batch() * s.rows * s.ld() * 2, ab = s.batch() * s.r() * s.ldr() * 2;
+    at[k] = {take(xb), it.steps > 1 ? take(xb) : 0, it.steps > 2 ? take(xb) : -1, take(ab), take(ab)};
   }
   const int64_t pat = take(partials * 8);
   auto ws = at::empty({bytes}, like.options().dtype(at::kByte));
@@ -652,7 +643,7 @@ at::Tensor make_workspace(std::vector<Shape>& shapes, const Iteration& it, int64
     Shape& s = shapes[k];
     s.x[0] = reinterpret_cast<__half*>(base + at[k][0]);
     s.x[1] = reinterpret_cast<__half*>(base + at[k][1]);
-    s.low = at[k][2] < 0 ? nullptr : base + at[k][2];
+    s.low = at[k][2] < 0 ? nullptr : reinterpret_cast<__half*>(base + at[k][2]);
     s.gram = reinterpret_cast<__half*>(base + at[k][3]);
     s.poly = reinterpret_cast<__half*>(base + at[k][4]);
   }
@@ -700,7 +691,6 @@ int fill_passes(PassArgs& a, const std::vector<Shape>& shapes, const MatTable& t
     g.block_end = (int)blocks;
     g.hi = s.x[0];
     g.low = s.low;
-    g.low_ld = (int)s.low_ld();
     // 4 elements at a time: whole rows of such pieces and aligned tables
     bool vec = s.cols % 4 == 0;
     for (int i = 0; i < g.batch; ++i)

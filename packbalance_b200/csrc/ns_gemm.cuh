@@ -16,10 +16,13 @@
 // iteration produces (|X| <= ~1.2, |A| <= ~1.5, |P| <= 3.5 in the 2-norm) in fp16's normal
 // range.  Accumulation is fp32.  Small singular values grow 3.4-fold per step, and with them
 // the rounding of X in the directions X hardly has: so the early iterates carry their
-// rounding error as a second matrix ``low`` (e4m3, scaled by 2^11, which makes it at most as large
-// as X's own fp16 values, 307 in magnitude: e4m3 reaches 448), which enters through the linear
-// term, X' = P hi + a low.  Simulated against 64 bits over Gaussian, low-rank and power-law
-// spectra the result is off by at most 3.1e-3 of its norm (``low`` in fp16 2.9e-3, without it 4e-2).
+// rounding error as a second fp16 matrix ``low`` (scaled by 2^11, which makes it about as large as
+// X's own values), which enters through the linear term, X' = P hi + a low.  Simulated against 64
+// bits over Gaussian matrices, power-law spectra and one to sixteen dominant directions plus noise,
+// the result is off by at most 3.7e-3 of its norm from 64 rows on (Gaussian 1.9e-3) and 5.2e-3
+// for 33 to 63 rows, where fewer roundings average out.  ``low`` in e4m3 takes 2 to 6 % less
+// time (the 100M model's update 1.69 instead of 1.77 ms) and is off by up to 5.1e-3 with one
+// dominant direction; without it 4e-2.
 //
 // Kernel structure: that of the CTA-pair GEMM (gemm_pair.cuh), whose barrier and abort
 // protocol is kept.  CG = 2: a pair of CTAs computes a 256 x 256 tile with cta_group::2; CG =
@@ -38,7 +41,6 @@
 #pragma once
 
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "gemm_pair.cuh"
 
@@ -47,7 +49,7 @@ namespace pb {
 enum NsMode : int {
   NS_GRAM = 0,   // out = alpha acc
   NS_POLY = 1,   // out = alpha acc + beta add + diag I
-  NS_APPLY = 2,  // out, low = split(alpha acc + beta add)  (``low_in``: the input's low part, or none)
+  NS_APPLY = 2,  // out, low = split(alpha acc + beta add)  (``add``: the input's low part, or none)
   NS_LAST = 3,   // bf16 result
   NS_STEP = 4,   // p = decay p - step alpha acc (fp32), and the bf16 copy of p
 };
@@ -59,8 +61,7 @@ constexpr float kNsLowScale = 2048.f;
 struct NsGroup {
   CUtensorMap a, b;      // operands: 64 x 64 boxes of fp16 [batch][rows][cols]
   CUtensorMap out, low;  // 32 x 32 boxes of the results
-  const __half* add;     // POLY: addend, indexed as the result
-  const uint8_t* low_in; // APPLY: addend (null: none)
+  const __half* add;     // POLY, APPLY: addend, indexed as the result (APPLY: the low part, or null)
   long add_batch;        // elements between the addend's matrices
   int add_ld;
   int M, N, K;
@@ -245,48 +246,6 @@ __device__ __forceinline__ void stage_f16(uint8_t* s, const float (&v)[32]) {
     *reinterpret_cast<uint4*>(s + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)) = q;
   }
 }
-// e4m3 of a pair of low parts, and back.
-__device__ __forceinline__ uint32_t pack_low2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ float2 unpack_low2(uint32_t v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xffffu), __NV_E4M3);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-// 32 low parts of this lane's row -> 32-byte row of a plain [32 x 32] byte box.
-__device__ __forceinline__ void stage_low(uint8_t* s, const float (&v)[32]) {
-  const int r = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = 16 * j + 4 * k;
-      w[k] = pack_low2(v[i], v[i + 1]) | pack_low2(v[i + 2], v[i + 3]) << 16;
-    }
-    *reinterpret_cast<uint4*>(s + r * 32 + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-// 32 low parts of this lane's row, columns [col, col + 32) (``ld``: padded, a multiple of 16).
-__device__ __forceinline__ void ns_load_low(const uint8_t* row, bool ok, int col, int ld, uint4 (&q)[2]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    q[j] = ok && col + 16 * j < ld ? __ldg(reinterpret_cast<const uint4*>(row + col) + j) : make_uint4(0, 0, 0, 0);
-}
-__device__ __forceinline__ void ns_add_low(float (&v)[32], const uint4 (&q)[2], float alpha, float beta) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t* w = &q[j].x;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float2 f = unpack_low2(w[k / 2] >> (k % 2 * 16));
-      const int i = 16 * j + 2 * k;
-      v[i] = alpha * v[i] + beta * f.x;
-      v[i + 1] = alpha * v[i + 1] + beta * f.y;
-    }
-  }
-}
-
 // 32 fp16 of this lane's row of the addend, columns [col, col + 32); pieces at or beyond ``ld``
 // (the padded row length, a multiple of 8) read as zero.
 __device__ __forceinline__ void ns_load_add(const __half* row, bool ok, int col, int ld, uint4 (&q)[4]) {
@@ -339,9 +298,9 @@ __device__ __forceinline__ void ns_prefetch(const NsArgs& a, const Step& sa, int
     const char* p = nullptr;
     int piece = 0;  // columns per 128-byte line
     if constexpr (MODE == NS_APPLY) {
-      if (g.low_in == nullptr) return;
-      p = reinterpret_cast<const char*>(g.low_in + t.mat * g.add_batch + static_cast<long>(row) * g.add_ld + col);
-      piece = 128;
+      if (g.add == nullptr) return;
+      p = reinterpret_cast<const char*>(g.add + t.mat * g.add_batch + static_cast<long>(row) * g.add_ld + col);
+      piece = 64;
     } else {
       p = reinterpret_cast<const char*>(sa.p[g.mat0 + t.mat] + static_cast<long>(row) * g.N + col);
       piece = 32;
@@ -365,17 +324,13 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
   const int col0 = t.j * C::T + c0;
   if constexpr (MODE == NS_GRAM || MODE == NS_POLY || MODE == NS_APPLY) {
     const bool ok = row < g.M;
-    const long at = t.mat * g.add_batch + static_cast<long>(ok ? row : 0) * g.add_ld;
-    uint4 q[MODE == NS_POLY ? W / 32 : 1][4];
-    uint4 lq[MODE == NS_APPLY ? W / 32 : 1][2];
-    if constexpr (MODE == NS_POLY) {
+    const bool with_add = MODE == NS_POLY || (MODE == NS_APPLY && g.add != nullptr);
+    uint4 q[MODE == NS_GRAM ? 1 : W / 32][4];
+    if constexpr (MODE != NS_GRAM) {
+      if (with_add) {
+        const __half* from = g.add + t.mat * g.add_batch + static_cast<long>(ok ? row : 0) * g.add_ld;
 #pragma unroll
-      for (int k = 0; k < W / 32; ++k) ns_load_add(g.add + at, ok, col0 + 32 * k, g.add_ld, q[k]);
-    }
-    if constexpr (MODE == NS_APPLY) {
-      if (g.low_in != nullptr) {
-#pragma unroll
-        for (int k = 0; k < W / 32; ++k) ns_load_low(g.low_in + at, ok, col0 + 32 * k, g.add_ld, lq[k]);
+        for (int k = 0; k < W / 32; ++k) ns_load_add(from, ok, col0 + 32 * k, g.add_ld, q[k]);
       }
     }
     if (!wait()) return false;
@@ -385,10 +340,9 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
       if (col >= g.N) break;  // uniform across the warp
       float v[32];
       tmem_load_f32(tacc + 32 * k, v);
-      if constexpr (MODE == NS_POLY) ns_add(v, q[k], a.alpha, a.beta);
-      if (MODE == NS_APPLY && g.low_in != nullptr) {
-        ns_add_low(v, lq[MODE == NS_APPLY ? k : 0], a.alpha, a.beta);
-      } else if (MODE != NS_POLY) {
+      if (with_add) {
+        ns_add(v, q[MODE == NS_GRAM ? 0 : k], a.alpha, a.beta);
+      } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= a.alpha;
       }
@@ -408,7 +362,7 @@ __device__ __forceinline__ bool ns_epilogue(const NsArgs& a, const Step& sa, con
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = (v[j] - __half2float(__float2half_rn(v[j]))) * kNsLowScale;
           s = st.acquire();
-          stage_low(s, v);
+          stage_f16(s, v);
           ns_store(&g.low, s, col, row0, t.mat);
           st.release();
         }
