@@ -6,6 +6,8 @@ odd polynomial steps.  ``muon_update_`` applies one Muon step to lists of matric
 The CUDA iteration keeps its operands in fp16 at fixed scales and accumulates in fp32; before
 the result is rounded to the output type it is within 4e-3 of the 64-bit iteration in the
 Frobenius norm (within 5.5e-3 for 33 to 63 rows or columns; up to 32 run in fp32 throughout).
+It takes up to 2 GB of workspace, or what the largest matrix needs (6 bytes per element and 4 per
+element of its smaller square); longer lists go through in parts.
 """
 
 from __future__ import annotations
