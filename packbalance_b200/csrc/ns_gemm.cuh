@@ -247,11 +247,12 @@ __device__ __forceinline__ void stage_f16(uint8_t* s, const float (&v)[32]) {
   }
 }
 // 32 fp16 of this lane's row of the addend, columns [col, col + 32); pieces at or beyond ``ld``
-// (the padded row length, a multiple of 8) read as zero.
+// (the padded row length, a multiple of 8) read as zero.  Coherent loads: APPLY stores the new low
+// part over the one that it reads here.
 __device__ __forceinline__ void ns_load_add(const __half* row, bool ok, int col, int ld, uint4 (&q)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    q[j] = ok && col + 8 * j < ld ? __ldg(reinterpret_cast<const uint4*>(row + col) + j) : make_uint4(0, 0, 0, 0);
+    q[j] = ok && col + 8 * j < ld ? *(reinterpret_cast<const uint4*>(row + col) + j) : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ void ns_add(float (&v)[32], const uint4 (&q)[4], float alpha, float beta) {
 #pragma unroll
