@@ -22,6 +22,12 @@ import torch
 from packbalance_b200.parallel.flat import FlatParameters
 
 
+def _check_entries(slot, state: dict[str, Any] | None, need: tuple[str, ...]) -> None:
+    missing = [k for k in need if state is not None and k not in state]
+    if missing:
+        raise ValueError(f"optimizer state of {slot.name} has no {missing}: written by another optimizer")
+
+
 class FlatAdamW(torch.optim.Optimizer):
     def __init__(
         self,
@@ -61,12 +67,14 @@ class FlatAdamW(torch.optim.Optimizer):
         saved_ids = groups[0]["params"]
         if len(saved_ids) != len(self.flat.slots):
             raise ValueError(f"optimizer state has {len(saved_ids)} params, model has {len(self.flat.slots)}")
+        states = [(s, state_dict["state"].get(pid)) for pid, s in zip(saved_ids, self.flat.slots, strict=True)]
+        for s, st in states:  # before anything changes
+            _check_entries(s, st, ("exp_avg", "exp_avg_sq"))
         for key, value in groups[0].items():
             if key != "params":
                 self.param_groups[0][key] = value
         steps = []
-        for pid, s in zip(saved_ids, self.flat.slots, strict=True):
-            st = state_dict["state"].get(pid)
+        for s, st in states:
             if st is None:
                 continue
             self.exp_avg[s.offset : s.offset + s.numel].copy_(st["exp_avg"].reshape(-1))
@@ -234,10 +242,7 @@ class FlatMuon(torch.optim.Optimizer):
         matrices = {id(s.param) for s in self.matrices}
         states = [(s, state_dict["state"].get(pid)) for pid, s in zip(saved_ids, self.flat.slots, strict=True)]
         for s, st in states:  # before anything changes
-            need = ("momentum_buffer",) if id(s.param) in matrices else ("exp_avg", "exp_avg_sq")
-            missing = [k for k in need if st is not None and k not in st]
-            if missing:
-                raise ValueError(f"optimizer state of {s.name} has no {missing}: written by another optimizer")
+            _check_entries(s, st, ("momentum_buffer",) if id(s.param) in matrices else ("exp_avg", "exp_avg_sq"))
         for key, value in groups[0].items():
             if key != "params":
                 self.param_groups[0][key] = value

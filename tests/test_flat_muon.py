@@ -104,6 +104,21 @@ def test_refuses_state_of_another_optimizer_and_bad_matrices(model_cfg: ModelCon
         FlatMuon(flat, [torch.nn.Parameter(torch.ones(2, 2))])
 
 
+def test_adamw_refuses_the_state_of_muon_before_anything_changes(model_cfg: ModelConfig) -> None:
+    _, flat, muon = _make(model_cfg)
+    flat.grad.fill_(1e-3)
+    muon.step()
+    adam = FlatAdamW(FlatParameters(LlamaForCausalLM(model_cfg)), lr=0.5)
+    kept = [t.clone() for t in (adam.exp_avg, adam.exp_avg_sq)], dict(adam.param_groups[0])
+    with pytest.raises(ValueError, match="another optimizer"):
+        adam.load_state_dict(muon.state_dict())
+    for got, want in zip((adam.exp_avg, adam.exp_avg_sq), kept[0]):
+        assert torch.equal(got, want)
+    assert {k: v for k, v in adam.param_groups[0].items() if k != "params"} == \
+        {k: v for k, v in kept[1].items() if k != "params"}
+    assert adam.step_count == 0
+
+
 def test_norm_type_builds_layer_norms(model_cfg: ModelConfig) -> None:
     model = LlamaForCausalLM(replace(model_cfg, norm_type="layernorm"))
     norms = [m for m in model.modules() if isinstance(m, LayerNorm)]
