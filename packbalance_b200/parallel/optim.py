@@ -307,8 +307,8 @@ class FlatMuon(torch.optim.Optimizer):
              hparams: torch.Tensor | None = None):
         """One update; arguments as :meth:`FlatAdamW.step`."""
         loss = closure() if closure is not None else None
-        if grad_norm is not None and not grad_norm.is_cuda:
-            if not torch.isfinite(grad_norm):
+        if not self.flat.data.is_cuda:
+            if grad_norm is not None and not torch.isfinite(grad_norm):
                 self.last_skipped.fill_(1)
                 return loss
             self.last_skipped.fill_(0)

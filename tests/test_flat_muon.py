@@ -74,6 +74,15 @@ def test_nonfinite_norm_skips_update(model_cfg: ModelConfig) -> None:
     assert not torch.equal(before, flat.data) and int(opt.last_skipped) == 0
 
 
+def test_a_step_without_a_norm_clears_the_skip(model_cfg: ModelConfig) -> None:
+    _, flat, opt = _make(model_cfg)
+    flat.grad.fill_(1.0)
+    opt.step(grad_norm=torch.tensor(math.inf), max_norm=1.0)
+    assert int(opt.last_skipped) == 1
+    opt.step()
+    assert int(opt.last_skipped) == 0 and opt.step_count == 1
+
+
 def test_checkpoint_round_trip_continues_the_run(tmp_path: Path, model_cfg: ModelConfig) -> None:
     model, flat, opt = _make(model_cfg)
     gen = torch.Generator().manual_seed(4)
