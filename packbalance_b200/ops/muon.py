@@ -12,6 +12,7 @@ element of its smaller square); longer lists go through in parts.
 
 from __future__ import annotations
 
+import bisect
 from collections.abc import Sequence
 
 import torch
@@ -31,6 +32,27 @@ def _check_iteration(steps: int, coefficients: Sequence[float], name: str) -> tu
     if len(coefficients) != 3:
         raise ValueError(f"{name}: three coefficients, got {len(coefficients)}")
     return tuple(float(c) for c in coefficients)
+
+
+def _check_memory(params, grads, momenta, shadows) -> None:
+    """What the native update checks of its arguments' memory: shadows of the right kind, nothing
+    that is written listed twice, and no gradient in it."""
+    for k, (w, p) in enumerate(zip(shadows, params)):
+        if w.dtype != torch.bfloat16 or w.device != p.device or w.numel() != p.numel() or not w.is_contiguous():
+            raise ValueError(f"muon_update_: shadow {k} must be contiguous bf16 of its parameter's size")
+
+    def spans(tensors):
+        return [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel()]
+
+    written = sorted(spans([*params, *momenta, *shadows]))
+    for (_, end), (start, _) in zip(written, written[1:]):
+        if end > start:
+            raise ValueError("muon_update_: parameters, momenta and shadows must not overlap or be listed twice")
+    for start, end in spans(grads):
+        # the written spans are disjoint: the one that starts last before ``end`` also ends last
+        k = bisect.bisect_left(written, (end,)) - 1
+        if k >= 0 and written[k][1] > start:
+            raise ValueError("muon_update_: gradients must not overlap parameters, momenta or shadows")
 
 
 @torch.no_grad()
@@ -105,6 +127,8 @@ def muon_update_(
             grad_norm, float(max_norm), hparams)
         torch.autograd.graph.increment_version([*params, *momenta, *(shadows or ())])
         return
+    grads = [g.contiguous() for g in grads]
+    _check_memory(params, grads, momenta, shadows or ())
     if hparams is not None:
         lr = float(hparams[0])
     scale = 1.0

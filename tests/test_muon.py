@@ -85,6 +85,50 @@ def test_refusals(call, message) -> None:
         call()
 
 
+_flat = torch.zeros(64)
+
+
+def _at(i, j):
+    return _flat[i:j].view(-1, 4)
+
+
+@pytest.mark.parametrize("p,g,m,shadows,message", [
+    ([_at(0, 12), _at(0, 12)], [_one(), _one()], [_one(), _one()], None, "listed twice"),
+    ([_at(0, 12), _at(8, 20)], [_one(), _one()], [_one(), _one()], None, "listed twice"),
+    ([_at(0, 12)], [_one()], [_at(8, 20)], None, "listed twice"),
+    ([_at(0, 12), _at(12, 24)], [_one(), _at(0, 12)], [_one(), _one()], None, "gradients must not overlap"),
+    ([_at(0, 12), _at(16, 28)], [_one(), _at(8, 20)], [_one(), _one()], None, "gradients must not overlap"),
+    ([_one()], [_at(0, 12)], [_at(0, 12)], None, "gradients must not overlap"),
+    ([_at(0, 12)], [_one()], [_one()], [_at(0, 12)], "bf16"),
+    ([_at(0, 12)], [_one()], [_one()], [torch.zeros(3, 3).bfloat16()], "size"),
+    ([_at(0, 12)], [_one()], [_one()], [torch.zeros(12)[4:10].view(torch.bfloat16).view(4, 3).t()], "contiguous"),
+])
+def test_cpu_update_refuses_what_the_native_one_refuses(p, g, m, shadows, message) -> None:
+    before = _flat.clone()
+    with pytest.raises(ValueError, match=message):
+        muon_update_(p, g, m, lr=0.1, shadows=shadows)
+    assert torch.equal(_flat, before)
+
+
+def test_cpu_update_of_neighbours_and_of_a_transposed_gradient() -> None:
+    """Parameters, momenta and gradients back to back in one buffer touch but do not overlap; a
+    transposed view of a parameter as gradient is read before anything is written."""
+    buf = torch.randn(48, generator=torch.Generator().manual_seed(5))
+    p, m, g = ([buf[k : k + 8].view(2, 4), buf[k + 8 : k + 16].view(4, 2)] for k in (0, 16, 32))
+    want = [t.clone() for t in p], [t.clone() for t in m]
+    muon_update_(want[0], [t.clone() for t in g], want[1], lr=0.1)
+    muon_update_(p, g, m, lr=0.1)
+    for got, expect in zip(p + m, want[0] + want[1]):
+        assert torch.equal(got, expect)
+    q = [torch.ones(2, 4), torch.randn(4, 2, generator=torch.Generator().manual_seed(6))]
+    n = [torch.zeros(2, 4), torch.zeros(4, 2)]
+    r, s = [t.clone() for t in q], [t.clone() for t in n]
+    muon_update_(r, [torch.ones(2, 4), r[0].clone().t()], s, lr=0.1)
+    muon_update_(q, [torch.ones(2, 4), q[0].t()], n, lr=0.1)
+    for got, expect in zip(q + n, r + s):
+        assert torch.equal(got, expect)
+
+
 def test_empty_lists_and_empty_matrices() -> None:
     muon_update_([], [], [], lr=0.1)
     assert orthogonalize(torch.ones(0, 3, 4)).shape == (0, 3, 4)
