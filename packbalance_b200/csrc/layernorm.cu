@@ -715,13 +715,17 @@ bool with_plan(int64_t n, F&& f) {
         return true;
       }
     };
-    // a row longer than 32 threads hold fills more than half of the pieces
+    // a row longer than 32 threads hold fills more than half of the pieces: half as many threads
+    // would hold it otherwise
     if constexpr (TT == 32) {
       if (try_k(std::integral_constant<int, most / 8>{}) || try_k(std::integral_constant<int, most / 4>{}) ||
           try_k(std::integral_constant<int, most / 2>{}))
         return true;
     }
-    return try_k(std::integral_constant<int, most * 3 / 4>{}) || try_k(std::integral_constant<int, most>{});
+    if constexpr (most * 3 / 4 > most / 2) {
+      if (try_k(std::integral_constant<int, most * 3 / 4>{})) return true;
+    }
+    return try_k(std::integral_constant<int, most>{});
   };
   return with_t(std::integral_constant<int, 32>{}) || with_t(std::integral_constant<int, 64>{}) ||
          with_t(std::integral_constant<int, 128>{}) || with_t(std::integral_constant<int, 256>{}) ||
@@ -871,6 +875,8 @@ at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor m
     check_act(*dx_bf16, x, "dx_bf16");
     TORCH_CHECK(dx_bf16->scalar_type() == at::kBFloat16, "layernorm: dx_bf16 must be bf16");
   }
+  TORCH_CHECK(x.scalar_type() == at::kFloat || (dy.scalar_type() == at::kBFloat16 && !dres.has_value() && !dx_bf16.has_value()),
+              "layernorm: a bf16 x has a bf16 dy, no dres and no dx_bf16");
   const c10::cuda::CUDAGuard guard(x.device());
   auto dx = at::empty_like(x);
   auto s = at::cuda::getCurrentCUDAStream();
@@ -903,30 +909,28 @@ at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor m
         });
       };
       constexpr bool XF = sizeof(TI) == 4, DF = sizeof(TD) == 4;
-      bool done = false;
-      if (rows > 0) {
+      if constexpr (XF || !DF) {  // checked above
+        const bool wide = n % (DF ? V : 8) == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) &&
+                          (dr == nullptr || aligned(*dres, 16)) && (dxb == nullptr || aligned(*dx_bf16, 8));
+        bool done = false;
         if constexpr (XF) {
-          const bool wide = n % (sizeof(TD) == 2 ? 8 : V) == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) &&
-                            (dr == nullptr || aligned(*dres, 16)) && (dxb == nullptr || aligned(*dx_bf16, 8));
-          if (dr != nullptr)
+          if (rows > 0 && dr != nullptr)
             done = wide ? launch(std::integral_constant<int, V>{}, std::true_type{})
                         : launch(std::integral_constant<int, 1>{}, std::true_type{});
-          else
+        }
+        // (the bf16 dy of an fp32 x comes with a residual gradient: the sum's two results)
+        if constexpr (XF == DF) {
+          if (rows > 0 && dr == nullptr)
             done = wide ? launch(std::integral_constant<int, V>{}, std::false_type{})
                         : launch(std::integral_constant<int, 1>{}, std::false_type{});
-        } else if constexpr (!DF) {
-          if (dr == nullptr && dxb == nullptr)
-            done = n % V == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16)
-                       ? launch(std::integral_constant<int, V>{}, std::false_type{})
-                       : launch(std::integral_constant<int, 1>{}, std::false_type{});
         }
+        if (done) return;
+        if (rows > 0)
+          ln_bwd_dx_kernel<<<rows, 256, 0, s>>>(dyp, xp, w.data_ptr<float>(), mean.data_ptr<float>(),
+                                                rstd.data_ptr<float>(), dr, dxp, dxb, (int)n);
+        ln_bwd_dw_kernel<<<(n + 31) / 32, 256, 0, s>>>(dyp, xp, mean.data_ptr<float>(), rstd.data_ptr<float>(),
+                                                       dw_out.data_ptr<float>(), dbp, (int)rows, (int)n, accumulate);
       }
-      if (done) return;
-      if (rows > 0)
-        ln_bwd_dx_kernel<<<rows, 256, 0, s>>>(dyp, xp, w.data_ptr<float>(), mean.data_ptr<float>(),
-                                              rstd.data_ptr<float>(), dr, dxp, dxb, (int)n);
-      ln_bwd_dw_kernel<<<(n + 31) / 32, 256, 0, s>>>(dyp, xp, mean.data_ptr<float>(), rstd.data_ptr<float>(),
-                                                     dw_out.data_ptr<float>(), dbp, (int)rows, (int)n, accumulate);
     });
   });
   PB_CUDA_CHECK(cudaGetLastError());

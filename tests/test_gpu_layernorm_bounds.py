@@ -140,3 +140,22 @@ def test_column_sums(rows, n, dtype):
         _near(dx[at : at + 1], one.dx, one.dx_tol)
         dx[at] = 0
         assert not dx.any()
+
+
+def test_native_backward_types():
+    """A bf16 dy of an fp32 x without a residual gradient takes the kernels of any width; what no
+    forward pass makes is refused."""
+    C = _native.module()
+    x, w, b, gen = _plain_rows(300, 768, torch.float32)
+    _, _, mean, rstd = C.add_layernorm_fwd(x, None, w, b, 1e-5, False)
+    dy = torch.randn(300, 768, generator=gen, device=dev).bfloat16()
+    dw, db, copy = torch.empty(768, device=dev), torch.empty(768, device=dev), torch.empty_like(dy)
+    dx = C.layernorm_bwd(dy, x, w, mean, rstd, None, copy, dw, db, False)
+    ex = _Exact(x, w, b, 1e-5, dy)
+    for got, want, tol in ((dx, ex.dx, ex.dx_tol), (dw, ex.dw, ex.dw_tol), (db, ex.db, ex.db_tol)):
+        _near(got, want, tol)
+    assert torch.equal(copy, dx.bfloat16())
+    half = x.bfloat16()
+    for args in ((dy.float(), None, None), (dy, x, None), (dy, None, copy)):
+        with pytest.raises(RuntimeError, match="bf16 x"):
+            C.layernorm_bwd(args[0], half, w, mean, rstd, args[1], args[2], dw, db, False)
