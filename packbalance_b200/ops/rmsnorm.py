@@ -15,7 +15,8 @@ class _RMSNorm(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1]).contiguous()
         y, rstd = _native.module().rmsnorm_fwd(x2, weight.float().contiguous(), float(eps), False)
         ctx.save_for_backward(x2, weight, rstd)
-        return y.reshape(x.shape)
+        # no view for autograd: torch refuses to change a view that a node returned in place
+        return y if y.shape == x.shape else torch.ops.aten._unsafe_view(y, x.shape)
 
     @staticmethod
     def backward(ctx, dy):

@@ -94,3 +94,18 @@ def test_graphs_of_the_sum_are_freed():
     for _ in range(4):
         add_layernorm(x, delta, w, b)
     assert torch.cuda.memory_allocated() <= before
+
+
+@pytest.mark.parametrize("shape", [(6, 64), (2, 3, 64), (64,)])
+def test_rmsnorm_results_change_in_place(shape):
+    from packbalance_b200.ops.rmsnorm import rmsnorm
+
+    x, _, w, _ = _tensors()
+    x = x.flatten()[: 384 if len(shape) > 1 else 64].view(shape)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    want = torch.autograd.grad(rmsnorm(*leaves, 1e-5), leaves, 2 * torch.ones_like(x))
+    y = rmsnorm(*leaves, 1e-5)
+    y.mul_(2.0)
+    assert y.shape == x.shape
+    for got, expect in zip(torch.autograd.grad(y, leaves, torch.ones_like(x)), want):
+        assert torch.equal(got, expect)
