@@ -10,7 +10,8 @@
 // rounding, so pass 1 updates the momentum and sums u^2 per 8192-element chunk, and pass 2
 // reads momentum and gradient again, adds up its matrix's chunk sums (in chunk order: no
 // atomics, the result does not depend on scheduling) and writes X0 as fp16 high and low parts.
-// Both are memory-bound (85M elements: 137 and 135 us, 7.4 TB/s and 6.9 TB/s).  The products follow
+// Both are memory-bound (the 100M model's 75.5M elements, 12 bytes each: 138 and 142 us, 6.6 and
+// 6.4 TB/s).  The products follow
 // as three launches per step (ns_gemm.cuh).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -218,7 +219,10 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const __grid_constant__ Pa
 // or in ``scratch`` when it does not fit), and run the whole update in one launch: momentum,
 // norm, every step, and the store.  The blocks' partial Gram matrices are added in block order
 // through distributed shared memory; the polynomial is computed by every block for itself.
-// Bound by latency: a 5-step 32 x 256 iteration is 15 dependent passes over 32 KB.
+// Bound by its passes over shared memory: the Gram phase reads 8 values per 16 multiply-adds, and
+// its 36 blocks of 32 rows make three uneven rounds of 16 warps; below a few thousand columns by
+// the latency of 15 dependent passes.  Measured: 1 x 32 x 768 78 us, 12 x 16 x 768 31 us,
+// 23 x 32 x 3232 202 us, 100 x 8 x 4096 89 us.
 //   Gram   a warp takes 4 x 4 blocks of row pairs, its lanes run along the long side
 //   apply  a thread takes one column: R values in registers, P from shared memory
 struct SmallArgs {

@@ -35,9 +35,10 @@
 //   warp 0 TMA producer, warp 1 TMEM allocation and MMA issue, warps 2-9 epilogue: two per
 //   quarter of the TMEM lanes, each finishing half of the tile's columns.
 //
-// Measured (B200, the 100M model's 84 matrices): GRAM 57 us (0.95 PFLOP/s of useful work), POLY
-// 45 us (K = 768 or less: epilogue and pipeline start), APPLY 97 us, 142 us where it reads and
-// writes low parts (HBM), STEP 172 us (HBM: 850 MB at 4.9 TB/s).
+// Measured (B200, the 100M model's 84 matrices, device time of a launch within the whole update): the
+// first GRAM 58 us (0.95 PFLOP/s of useful work), the later ones, under the power cap, 72 to 84; POLY
+// 57 to 64 us (K = 768 or less: epilogue and pipeline start); APPLY 107 us, 170 where it reads and
+// writes low parts (604 MB at 3.6 TB/s); STEP 176 us (755 MB at 4.3 TB/s).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -285,8 +286,9 @@ __device__ __forceinline__ float ns_block_at(const float* s, int r, int c) {
 }
 
 // What the epilogue of ``tile`` will read for this warp's rows (the low part, the parameters)
-// starts moving into L2 while the tile before it is finished: both are larger than L2 and the
-// DRAM latency was otherwise paid once per 32 columns.
+// starts moving into L2 while the tile before it is finished: the parameters, and the low parts of
+// all matrices together, are larger than L2, and the DRAM latency was otherwise paid once per 32
+// columns.
 template <int CG, int MODE, class Step>
 __device__ __forceinline__ void ns_prefetch(const NsArgs& a, const Step& sa, int tile, int row_in_tile, int c0) {
   using C = NsCfg<CG>;

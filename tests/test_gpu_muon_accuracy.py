@@ -62,3 +62,24 @@ def test_one_to_sixteen_dominant_directions(batch, m, n, rank, noise):
     print(f"{batch}x{m}x{n} rank {rank} + {noise}: {off:.2e}")
     assert off <= bound
     assert _off(orthogonalize(u), want) <= math.hypot(bound, 2.0**-8)
+
+
+@pytest.mark.parametrize("scale", [1e-9, 1e-11, 1e-13])
+@pytest.mark.parametrize("m,n", [(64, 200), (256, 768), (1024, 1024)])
+def test_matrices_far_smaller_than_eps(m, n, scale):
+    """Down to |x|_F = 1e-6 eps the carried rounding errors hold what fp16 loses (simulated: 2.1e-3)."""
+    x = torch.randn(2, m, n, generator=torch.Generator(device=dev).manual_seed(n), device=dev)
+    x = x / torch.linalg.matrix_norm(x, keepdim=True) * scale
+    p, mom = torch.zeros_like(x), torch.zeros_like(x)
+    muon_update_([p], [x], [mom], lr=1.0 / (0.2 * math.sqrt(max(m, n))), momentum=0.0, nesterov=False, weight_decay=0.0)
+    assert _off(-p, _exact(x)) <= WIDE
+
+
+def test_the_largest_iterates_that_do_not_overflow():
+    """Singular values of 7.9 before the last step: A stays below 64.  Each of the three steps rounds
+    its factor and its iterate by at most 2^-11 together with the Gram matrix not entering."""
+    q = torch.linalg.qr(torch.randn(128, 128, generator=torch.Generator(device=dev).manual_seed(1), device=dev))[0]
+    a = (7.9 * 128**0.5) ** 0.5
+    y = orthogonalize(q, steps=3, coefficients=(a, 0.0, 0.0))
+    _native.check_status()
+    assert _off(y, a**3 * q.double() / 128**0.5) <= 3 * 2 * 2.0**-11 + 2.0**-8
