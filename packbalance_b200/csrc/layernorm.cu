@@ -32,12 +32,17 @@ __device__ __forceinline__ void stf(__nv_bfloat16* p, float v) { *p = __float2bf
 // ---- rows held in registers --------------------------------------------------------
 // T threads hold a row, K pieces of V elements each, so a row is read once; rows are dealt to a
 // persistent grid.  Weight, bias and the backward's column sums stay in registers over all of a
-// thread's rows.  Both directions wait for HBM only, and what has to be right for that is bytes
+// thread's rows.  What bounds both directions is HBM, and what has to be right for that is bytes
 // in flight.  Rows whose every operand starts on a 16-byte boundary arrive by bulk copies in a
 // ring of shared-memory slots (RING), several rows ahead; other rows come one element at a time
 // through registers (V = 1), one row ahead.
-// Measured (B200): 16384 x 4096 bf16 forward 47 us (5.7 TB/s, 0.87 of the measured copy), backward
-// 77 us (5.2 TB/s); 8192 x 768 with the residual add 13.5 and 15 us (5.6 and 6.5 TB/s, partly L2).
+// Measured (B200): 16384 x 4096 bf16 forward 51.5 us (5.2 TB/s, 0.80 of the measured copy), backward
+// with the column sums 82 us (4.9 TB/s); 8192 x 768 with the residual add 14.6 us (5.2 TB/s, partly L2),
+// its backward from an fp32 dy 24.7 us; 4001 x 1409 fp32 12.5 and 18 us.
+// The backward holds weight, column sums, xh and g besides the row: at 512 threads with a residual
+// gradient (above 6144 columns) and at 1024 (above 8192) not all of that fits, and it spills:
+// 16384 x 8192 fp32 with a residual gradient 507 us (4.2 TB/s; bf16 without one 150 us, 5.4 TB/s),
+// 8192 x 12288 fp32 420 us (2.9 TB/s), bf16 1050 us (0.6 TB/s).
 //
 // Arithmetic is on pairs of fp32 (one instruction each on sm_100a): one element at a time the
 // kernels issued 18 and 25 instructions per element and waited for those, not for HBM.
