@@ -896,7 +896,8 @@ at::Tensor layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor m
     check_act(*dx_bf16, x, "dx_bf16");
     TORCH_CHECK(dx_bf16->scalar_type() == at::kBFloat16, "layernorm: dx_bf16 must be bf16");
   }
-  TORCH_CHECK(x.scalar_type() == at::kFloat || (dy.scalar_type() == at::kBFloat16 && !dres.has_value() && !dx_bf16.has_value()),
+  TORCH_CHECK(x.scalar_type() == at::kFloat ||
+                  (dy.scalar_type() == at::kBFloat16 && !dres.has_value() && !dx_bf16.has_value()),
               "layernorm: a bf16 x has a bf16 dy, no dres and no dx_bf16");
   const c10::cuda::CUDAGuard guard(x.device());
   auto dx = at::empty_like(x);
